@@ -486,6 +486,121 @@ int qf_packed_rope_decode_attention(const qf_decode_attention_args* args, const 
  * kernels' formula.  `table` holds positions * 64 * 2 floats. */
 int qf_build_rope_table(float* table, int32_t positions, double base, void* stream);
 
+/* ------------------------------------------------------------------------
+ * 4-bit paged KV cache.  No counterpart in the reference; the layout is defined here.
+ *
+ * pool: bytes [num_pages][kv_heads][page_size / 16][20 * D], 16-byte aligned, contiguous;
+ * D = 64 or 128, page_size a multiple of 16.  A tile is 16 tokens of one KV head, K and V
+ * together.  Every 32 consecutive channels of a token's row are a group with a step and a
+ * floor of the queries' type T; a channel is a code n in 0..15 and stands for
+ * n * step + floor:
+ *   floor = min(x)   step = T((max(x) - min(x)) / 15)   n = clamp(rint((x - floor) / step))
+ * in fp32 with IEEE divisions, 5 bits a channel in all.  A step below 2^-60 is held as 0.
+ * A group that holds an infinity or a NaN reads back as NaN.  Bytes of a tile, W = D / 32:
+ *   [0, 8D)     K codes [16 tokens][4 t][W][4]: byte y of (t, w): channels 32w + 8t + 2y (low
+ *               four bits) and 32w + 8t + 2y + 1
+ *   [8D, 16D)   V codes [8 token pairs][8 g][W][2 tokens][2]: byte y of (g, w): channels
+ *               32w + 4g + 2y and 32w + 4g + 2y + 1
+ *   [16D, 20D)  K steps [16][W], K floors [16][W], V steps [16][W], V floors [16][W]
+ * Token p of a sequence is in page block_table[p / page_size], tile (p % page_size) / 16.
+ * ------------------------------------------------------------------------ */
+
+/* RoPE + quantising cache write: qf_rope_kv_write for this cache (same strides, the same
+ * zero queries for rows >= *valid_tokens).  q_heads 0: only K and V.  positions NULL: K is
+ * stored as it is (and Q, if any, copied).  rope_table [table_positions][D / 2] (cos, sin)
+ * fp32 pairs, or NULL: cosf / sinf of position * base^(-2i / D) as in qf_rope_kv_write; a
+ * position outside the table is clamped and recorded (status 4).  A rotated key is rounded
+ * to T and then quantised.  slot_mapping NULL: slot = row.  A slot outside the pool is
+ * skipped.  Two rows of one call with the same slot leave a mixture of both in it. */
+typedef struct qf_int4_write_args {
+  const void* q; /* device, may be NULL when q_heads == 0 */
+  const void* k;
+  const void* v;
+  void* q_out;
+  int64_t q_stride_row, q_stride_head, q_stride_d;
+  int64_t k_stride_row, k_stride_head, k_stride_d;
+  int64_t v_stride_row, v_stride_head, v_stride_d;
+  int64_t o_stride_row, o_stride_head, o_stride_d;
+  const void* positions; /* device [rows] or NULL */
+  int64_t positions_stride;
+  const void* slot_mapping; /* device [rows] or NULL */
+  int64_t slot_stride;
+  const float* rope_table; /* device or NULL */
+  void* pool;
+  int64_t num_pages;
+  const int32_t* valid_tokens; /* device scalar or NULL */
+  int32_t rows, q_heads, kv_heads, head_dim;
+  int32_t page_size, dtype;
+  int32_t positions_dtype, slot_dtype; /* QF_INDEX_* */
+  int32_t table_positions;
+  double base;
+} qf_int4_write_args;
+int qf_int4_rope_kv_write(const qf_int4_write_args* args, void* stream);
+
+/* Rows of the cache at a list of slots (NULL: slot = row) as 16-bit K and V, both
+ * [rows, kv_heads, D] contiguous: T(n * step + floor), the sum rounded in fp32 first.  A
+ * slot outside the pool gives a row of zeros. */
+int qf_int4_read_rows(const void* pool, int64_t num_pages, int32_t page_size, int32_t kv_heads,
+                      int32_t head_dim, int32_t dtype, const void* slots, int32_t slot_dtype,
+                      int64_t slot_stride, int64_t rows, void* k_out, void* v_out, void* stream);
+
+/* Arguments of the calls that walk block tables of this cache.  A row is a (sequence, KV
+ * head); table_stride_h / lens_stride_h 0: the KV heads of a sequence share table and length.
+ * A length below 0 counts as 0, one beyond the table's width as that.  q and out
+ * [batch, q_heads, D]: unit inner stride, 16-byte aligned, other strides multiples of 8;
+ * q_heads / kv_heads at most 16.  A page id outside the pool is never dereferenced: it is
+ * recorded (status 2), its tokens read as zeros. */
+typedef struct qf_paged_int4_args {
+  const void* q;
+  void* out;
+  const void* pool;
+  void* key_bounds; /* T [num_pages, kv_heads, 2, D]: smallest, largest key of a page, per channel */
+  const void* block_table;
+  const void* seq_lens;
+  void* workspace; /* device scratch of this call, qf_paged_int4_workspace bytes, 16-byte aligned */
+  int32_t* page_table; /* device [batch, kv_heads, take]: the pages chosen */
+  int32_t* page_lens;  /* device [batch, kv_heads]: the tokens they hold */
+  int64_t q_stride_b, q_stride_h, o_stride_b, o_stride_h;
+  int64_t table_stride_b, table_stride_h, table_stride_p, lens_stride_b, lens_stride_h;
+  int64_t num_pages, table_width, workspace_bytes;
+  int32_t batch, q_heads, kv_heads, head_dim, page_size, dtype;
+  int32_t table_dtype, lens_dtype;
+  int32_t new_tokens; /* qf_int4_key_bounds */
+  int32_t take;       /* qf_select_kv_pages, qf_int4_sparse_decode_attention */
+  float scale;        /* softmax scale */
+} qf_paged_int4_args;
+
+#define QF_INT4_ATTENTION 0
+#define QF_INT4_SELECT 1
+#define QF_INT4_SPARSE 2
+/* Scratch bytes of qf_int4_decode_attention, qf_select_kv_pages or
+ * qf_int4_sparse_decode_attention (`call`, above) for these arguments on the current device.
+ * Reads no device memory; nothing in the scratch needs clearing, and none of it may be shared
+ * by calls that can overlap on the GPU. */
+int qf_paged_int4_workspace(const qf_paged_int4_args* args, int32_t call, int64_t* bytes);
+
+/* out = softmax(scale * q k) v over every row's tokens; a row of length 0 gives zeros. */
+int qf_int4_decode_attention(const qf_paged_int4_args* args, void* stream);
+
+/* key_bounds of every page that holds one of the last `new_tokens` tokens of its sequence,
+ * over the page's tokens below the sequence's length; other pages keep theirs.  Table and
+ * lengths are those of the sequences (the head strides are not used).  A NaN key makes both
+ * bounds of its channel NaN. */
+int qf_int4_key_bounds(const qf_paged_int4_args* args, void* stream);
+
+/* The pages every row attends: its newest page and the take - 1 others with the highest
+ *   score = max over the KV head's query heads of sum_d max(q_d * low_d, q_d * high_d)
+ * (fp32, products exact, summed pairwise with neighbouring channels first; ties to the lower
+ * page of the sequence, a NaN above every number).  page_table: their ids in the sequence's
+ * order, the newest last, -1 behind them when the sequence has fewer; page_lens: the tokens
+ * they hold -- a block table and lengths with head strides for qf_int4_decode_attention.  A
+ * page id outside the pool scores below every other.  Table and lengths are those of the
+ * sequences.  batch * kv_heads at most 65535.  Ends with qf_order_next_launch(). */
+int qf_select_kv_pages(const qf_paged_int4_args* args, void* stream);
+
+/* qf_select_kv_pages, then qf_int4_decode_attention over the pages it chose. */
+int qf_int4_sparse_decode_attention(const qf_paged_int4_args* args, void* stream);
+
 /* Switches for tests and experiments (process-wide, read at launch time).
  * force_generic: 0 automatic choice; 1 every attention call goes through the
  * stride-generic kernel; 2 fast per-partition kernel only, no persistent kernel;

@@ -21,6 +21,12 @@ current torch stream; none has a CPU fallback):
     native_decode_rope_kv_write_fp8, packed_qkv_rope_cache_fp8,
     grouped_splitk_decode_attention_fp8,
     packed_qkv_rope_attention_fp8                          custom_kernels/fp8_paged_kv.py
+    empty_kv_pool_int4, quantize_kv_pool_int4, dequantize_kv_pool_int4,
+    rope_kv_write_int4, native_decode_rope_kv_write_int4,
+    packed_qkv_rope_cache_int4, read_kv_int4,
+    paged_decode_attention_int4, empty_key_bounds_int4,
+    update_key_bounds_int4, select_kv_pages,
+    sparse_decode_attention_int4                           custom_kernels/int4_paged_kv.py
     advance_decode_state                                   custom_kernels/decode_state.py
     rms_norm, residual_add_rms_norm                        custom_kernels/fused_rms.py
     qkv_rope_cache, qkv_rope_cache_timeline                custom_kernels/fused_gemm.py
@@ -55,6 +61,18 @@ _EXPORTS = {
     "packed_qkv_rope_cache_fp8": "fp8_paged_kv",
     "grouped_splitk_decode_attention_fp8": "fp8_paged_kv",
     "packed_qkv_rope_attention_fp8": "fp8_paged_kv",
+    "empty_kv_pool_int4": "int4_paged_kv",
+    "quantize_kv_pool_int4": "int4_paged_kv",
+    "dequantize_kv_pool_int4": "int4_paged_kv",
+    "rope_kv_write_int4": "int4_paged_kv",
+    "native_decode_rope_kv_write_int4": "int4_paged_kv",
+    "packed_qkv_rope_cache_int4": "int4_paged_kv",
+    "read_kv_int4": "int4_paged_kv",
+    "paged_decode_attention_int4": "int4_paged_kv",
+    "empty_key_bounds_int4": "int4_paged_kv",
+    "update_key_bounds_int4": "int4_paged_kv",
+    "select_kv_pages": "int4_paged_kv",
+    "sparse_decode_attention_int4": "int4_paged_kv",
     "advance_decode_state": "decode_state",
     "rms_norm": "fused_rms",
     "residual_add_rms_norm": "fused_rms",

@@ -36,12 +36,14 @@ EXPORTED_SYMBOLS = (
     "qf_set_dependent_launch", "qf_order_next_launch", "qf_advance_decode_metadata",
     "qf_rms_norm", "qf_residual_add_rms_norm", "qf_qkv_rope_cache",
     "qf_qkv_rope_cache_timeline", "qf_packed_rope_decode_attention",
-    "qf_build_rope_table",
+    "qf_build_rope_table", "qf_int4_rope_kv_write", "qf_int4_read_rows", "qf_paged_int4_workspace",
+    "qf_int4_decode_attention", "qf_int4_key_bounds", "qf_select_kv_pages", "qf_int4_sparse_decode_attention",
 )
 KERNEL_NAMES = ("decode_partial_kernel", "decode_stream_kernel", "decode_mma_kernel", "decode_mma_kernel (solo)")
 STAGE_PARTIAL, STAGE_COMBINE = 1, 2
 GEMM_TIMELINE_COLUMNS = 10
 STATIC_SCRATCH_BYTES = 16 << 20
+INT4_ATTENTION, INT4_SELECT, INT4_SPARSE = 0, 1, 2
 
 
 class RopeKvWriteArgs(Structure):
@@ -109,6 +111,46 @@ class QkvRopeCacheArgs(Structure):
     ]
 
 
+class Int4WriteArgs(Structure):
+    """Mirror of qf_int4_write_args."""
+
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_out", c_void_p),
+        ("q_stride_row", c_int64), ("q_stride_head", c_int64), ("q_stride_d", c_int64),
+        ("k_stride_row", c_int64), ("k_stride_head", c_int64), ("k_stride_d", c_int64),
+        ("v_stride_row", c_int64), ("v_stride_head", c_int64), ("v_stride_d", c_int64),
+        ("o_stride_row", c_int64), ("o_stride_head", c_int64), ("o_stride_d", c_int64),
+        ("positions", c_void_p), ("positions_stride", c_int64),
+        ("slot_mapping", c_void_p), ("slot_stride", c_int64),
+        ("rope_table", c_void_p), ("pool", c_void_p), ("num_pages", c_int64),
+        ("valid_tokens", c_void_p),
+        ("rows", c_int32), ("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+        ("page_size", c_int32), ("dtype", c_int32),
+        ("positions_dtype", c_int32), ("slot_dtype", c_int32),
+        ("table_positions", c_int32),
+        ("base", c_double),
+    ]
+
+
+class PagedInt4Args(Structure):
+    """Mirror of qf_paged_int4_args."""
+
+    _fields_ = [
+        ("q", c_void_p), ("out", c_void_p), ("pool", c_void_p), ("key_bounds", c_void_p),
+        ("block_table", c_void_p), ("seq_lens", c_void_p), ("workspace", c_void_p),
+        ("page_table", c_void_p), ("page_lens", c_void_p),
+        ("q_stride_b", c_int64), ("q_stride_h", c_int64), ("o_stride_b", c_int64), ("o_stride_h", c_int64),
+        ("table_stride_b", c_int64), ("table_stride_h", c_int64), ("table_stride_p", c_int64),
+        ("lens_stride_b", c_int64), ("lens_stride_h", c_int64),
+        ("num_pages", c_int64), ("table_width", c_int64), ("workspace_bytes", c_int64),
+        ("batch", c_int32), ("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+        ("page_size", c_int32), ("dtype", c_int32),
+        ("table_dtype", c_int32), ("lens_dtype", c_int32),
+        ("new_tokens", c_int32), ("take", c_int32),
+        ("scale", c_float),
+    ]
+
+
 _library = None
 
 
@@ -167,6 +209,13 @@ def library():
     lib.qf_packed_rope_decode_attention.argtypes = [
         POINTER(DecodeAttentionArgs), c_void_p, c_int32, c_int64, c_void_p, c_int32, c_int32, c_void_p]
     lib.qf_build_rope_table.argtypes = [c_void_p, c_int32, c_double, c_void_p]
+    lib.qf_int4_rope_kv_write.argtypes = [POINTER(Int4WriteArgs), c_void_p]
+    lib.qf_int4_read_rows.argtypes = (
+        [c_void_p, c_int64] + [c_int32] * 4 + [c_void_p, c_int32, c_int64, c_int64] + [c_void_p] * 3)
+    lib.qf_paged_int4_workspace.argtypes = [POINTER(PagedInt4Args), c_int32, POINTER(c_int64)]
+    for name in ("qf_int4_decode_attention", "qf_int4_key_bounds", "qf_select_kv_pages",
+                 "qf_int4_sparse_decode_attention"):
+        getattr(lib, name).argtypes = [POINTER(PagedInt4Args), c_void_p]
     for name in EXPORTED_SYMBOLS:
         if name not in ("qf_last_error",):
             getattr(lib, name).restype = c_int32
