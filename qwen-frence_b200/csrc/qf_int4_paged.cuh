@@ -31,7 +31,7 @@ struct PagedInt4 {
 enum : int { kNeedsQuery = 1, kNeedsPool = 2, kNeedsOut = 4, kNeedsBounds = 8, kNeedsSelection = 16 };
 
 int fill_paged_int4(const qf_paged_int4_args* args, int needs, PagedInt4* p);
-int64_t int4_attention_bytes(const PagedInt4& p);  // scratch of launch_int4_attention
+int64_t int4_attention_bytes(const PagedInt4& p, int head_dim);  // scratch of launch_int4_attention
 int launch_int4_attention(const PagedInt4& p, int head_dim, int dtype, cudaStream_t stream);
 
 // Tokens of row (b, h): never negative, never more than its table row can hold.
@@ -43,15 +43,6 @@ __device__ __forceinline__ int64_t row_tokens(const PagedInt4& p, int b, int h) 
 
 __device__ __forceinline__ int64_t page_id(const PagedInt4& p, int b, int h, int64_t n) {
   return load_index(p.table, p.table_dtype, b * p.t_sb + h * p.t_sh + n * p.t_sp);
-}
-
-// Address of tile `tile` (16 tokens) of row (b, h); null when its page is not in the pool.
-template <int D>
-__device__ __forceinline__ const uint8_t* tile_address(const PagedInt4& p, int b, int h, int64_t tile) {
-  const int per_page = p.page_size / kInt4Tile;
-  const int64_t page = page_id(p, b, h, tile / per_page);
-  if (page < 0 || page >= p.num_pages) return nullptr;
-  return p.pool + ((page * p.kv_heads + h) * per_page + tile % per_page) * int4_tile_bytes(D);
 }
 
 }  // namespace qf

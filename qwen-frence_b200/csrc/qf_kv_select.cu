@@ -17,6 +17,8 @@ int fill_paged_int4(const qf_paged_int4_args* a, int needs, PagedInt4* p) {
   QF_REQUIRE(a->batch >= 0 && a->kv_heads >= 1, "batch and head counts must be positive");
   QF_REQUIRE(static_cast<int64_t>(a->batch) * a->kv_heads < (1LL << 31), "too many rows");
   QF_REQUIRE(a->num_pages >= 0 && a->num_pages < (1LL << 31) && a->table_width >= 0, "invalid pool or table size");
+  // tiles of the pool are counted in 32 bits
+  QF_REQUIRE(a->num_pages <= 0xfffffffeLL / a->kv_heads / (a->page_size / kInt4Tile), "invalid pool or table size");
   // tokens of a row are counted in 32 bits
   QF_REQUIRE(a->table_width <= ((1LL << 31) - 1) / a->page_size, "a block table row holds 2^31 tokens or more");
   if (needs & kNeedsQuery) {
@@ -342,7 +344,7 @@ int qf_int4_sparse_decode_attention(const qf_paged_int4_args* args, void* stream
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   PagedInt4 next = over_selection(p);
   const int64_t keys = select_bytes(p);
-  const int64_t more = int4_attention_bytes(next);
+  const int64_t more = int4_attention_bytes(next, args->head_dim);
   QF_REQUIRE(p.workspace != nullptr && p.workspace_bytes >= keys + more, "the workspace holds %lld bytes, %lld are needed",
              static_cast<long long>(p.workspace_bytes), static_cast<long long>(keys + more));
   if (const int rc = launch_select(p, args->head_dim, args->dtype, s)) return rc;
@@ -361,7 +363,7 @@ int qf_paged_int4_workspace(const qf_paged_int4_args* args, int32_t call, int64_
   QF_REQUIRE(p.batch >= 0 && p.kv_heads >= 1 && p.q_heads >= 0 && p.table_width >= 0 && p.page_size >= 1, "invalid sizes");
   *bytes = 0;
   if (call != QF_INT4_ATTENTION) *bytes += select_bytes(p);
-  if (call != QF_INT4_SELECT) *bytes += int4_attention_bytes(call == QF_INT4_SPARSE ? over_selection(p) : p);
+  if (call != QF_INT4_SELECT) *bytes += int4_attention_bytes(call == QF_INT4_SPARSE ? over_selection(p) : p, args->head_dim);
   return QF_OK;
 }
 
