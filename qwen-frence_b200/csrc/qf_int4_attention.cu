@@ -25,21 +25,22 @@
 namespace qf {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = 32 * kWarps;
-constexpr uint32_t kBadTile = 0xffffffffu;
+constexpr int kUnit = 2 * kInt4Tile;  // tokens a warp takes at a time: two tiles, for the distance between dependent steps
+constexpr uint32_t kNoTile = 0xffffffffu;
+constexpr int kRowStart = 1, kRowEnd = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Bytes of shared memory of a warp's ring, and tiles in it.
 template <int D, int NT>
 struct Shape {
+  static constexpr int kWarps = NT == 1 ? 16 : 8;
+  static constexpr int kThreads = 32 * kWarps;
   static constexpr int kTileBytes = 20 * D;
-  static constexpr int kStages = (NT == 1 ? 12800 : 25600) / kTileBytes;  // D 128: 5 or 10, D 64: 10 or 20
-  static constexpr int kRing = kStages * kTileBytes;
+  static constexpr int kStageBytes = 2 * kTileBytes;
+  static constexpr int kStages = 208 * 1024 / kWarps / kStageBytes;  // of a warp's ring: one less in flight
+  static constexpr int kRing = kStages * kStageBytes;
   static constexpr int kHeads = 8 * NT;        // query heads a row has room for
   static constexpr int kStride = D + 4;        // floats between heads of a piece: its float4 stores miss no bank
   static constexpr int kPiece = kHeads * kStride + 2 * kHeads;  // floats: o, then offset and sum of every head
-  static constexpr int kCtasPerSm = NT == 1 ? 2 : 1;
   static constexpr int kSmem = kWarps * kRing;
   static_assert(kPiece * 4 <= kRing, "a piece fits its warp's ring");
 };
@@ -73,106 +74,158 @@ __device__ __forceinline__ float pow2i(int e) {  // 2^e, e in [-126, 127]
   return __int_as_float((e + 127) << 23);
 }
 
-__device__ __forceinline__ bool wait_stage(uint32_t bar, uint32_t parity) {
-  for (int spin = 0; spin < (1 << 20); ++spin) {
-    uint32_t done;
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                 : "=r"(done)
-                 : "r"(bar), "r"(parity)
-                 : "memory");
-    if (done) return true;
-  }
-  return false;
+// 16 bytes to shared memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// What a call shares out: tiles of all rows, tiles of a CTA.
+__device__ __forceinline__ uint64_t pair32(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair32(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+// Two products, or products and sums, in one instruction.
+__device__ __forceinline__ uint64_t mul32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// What a call shares out: units of all rows (fewer than 2^31), units of a CTA.
 struct Plan {
-  int64_t units;
-  int64_t share;
+  int units;
+  int share;
 };
 
-// Thread-chunk prefix sums of the rows' tiles: s_prefix[i] = tiles before thread i's rows.
-__device__ __forceinline__ Plan make_plan(const PagedInt4& p, int64_t* s_prefix, int64_t* s_warp, int chunk, int ctas) {
+__device__ __forceinline__ int row_tokens_at(const PagedInt4& p, int row) {
+  const int2 at = row_place(p, row);
+  return static_cast<int>(row_tokens(p, at.x, at.y));
+}
+
+// Shared by a CTA's warps: prefix sums of the rows' units, thread by thread (`chunk` rows each),
+// and, where a thread has one row, the rows' lengths.
+template <int kWarps>
+struct Shares {
+  int prefix[32 * kWarps];
+  int tokens[32 * kWarps];
+  int warp[kWarps];
+};
+
+template <int kWarps>
+__device__ __forceinline__ Plan make_plan(const PagedInt4& p, Shares<kWarps>& s, int chunk, int ctas) {
   const int rows = p.batch * p.kv_heads;
-  const int first = threadIdx.x * chunk;
-  int64_t mine = 0;
-  for (int r = first; r < first + chunk && r < rows; ++r) mine += (row_tokens(p, r / p.kv_heads, r % p.kv_heads) + kInt4Tile - 1) / kInt4Tile;
-  int64_t sum = mine;
+  const int first = threadIdx.x * chunk, lane = threadIdx.x & 31;
+  int mine = 0;
+  for (int r = first; r < first + chunk && r < rows; ++r) {
+    const int tokens = row_tokens_at(p, r);
+    mine += (tokens + kUnit - 1) / kUnit;
+    s.tokens[threadIdx.x] = tokens;
+  }
+  int sum = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, sum, off);
-    if ((threadIdx.x & 31) >= off) sum += up;
+    const int up = __shfl_up_sync(0xffffffffu, sum, off);
+    if (lane >= off) sum += up;
   }
-  if ((threadIdx.x & 31) == 31) s_warp[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  int64_t before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < (threadIdx.x >> 5)) before += s_warp[w];
-    total += s_warp[w];
-  }
-  s_prefix[threadIdx.x] = before + sum - mine;
+  if (lane == 31) s.warp[threadIdx.x >> 5] = sum;
+  s.prefix[threadIdx.x] = sum - mine;  // within the warp's rows
   __syncthreads();
   Plan plan;
-  plan.units = total;
-  plan.share = (total + ctas - 1) / ctas;
-  if (plan.share < kWarps) plan.share = kWarps;  // a tile a warp at least: fewer pieces for the second kernel
+  plan.units = __reduce_add_sync(0xffffffffu, lane < kWarps ? s.warp[lane] : 0);
+  plan.share = (plan.units + ctas - 1) / ctas;
+  if (plan.share < kWarps) plan.share = kWarps;  // a unit a warp at least: fewer pieces for the second kernel
   return plan;
 }
 
-// Tiles of 32 units ahead: lane i holds the tile, the tokens in it and the row of unit i.
-struct Batch {
-  uint32_t tile;
-  int meta;  // tokens 1..16, kRowStart, kRowEnd
-  int row;
-};
-constexpr int kRowStart = 32, kRowEnd = 64;
-
-struct Walk {
-  int row;    // next unit's row and tile in the row
-  int tile;
-  int left;   // units not described yet
-  int base;   // row of lane 0's length
-  int length; // tokens of row base + lane
-};
-
-__device__ __forceinline__ void load_lengths(const PagedInt4& p, Walk& w, int lane) {
-  const int rows = p.batch * p.kv_heads;
-  w.base = w.row;
-  const int r = w.row + lane;
-  w.length = r < rows ? static_cast<int>(row_tokens(p, r / p.kv_heads, r % p.kv_heads)) : 0;
+// The thread whose rows hold unit `first`, and the units before those rows.
+template <int kWarps>
+__device__ __forceinline__ int2 find_rows(const Shares<kWarps>& s, int first, int lane) {
+  const int mine = lane < kWarps ? s.warp[lane] : 0;
+  int sum = mine;
+#pragma unroll
+  for (int off = 1; off < kWarps; off <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, sum, off);
+    if (lane >= off) sum += up;
+  }
+  const int warp = __popc(__ballot_sync(0xffffffffu, lane < kWarps && sum <= first));  // warps that end before it
+  const int before = __shfl_sync(0xffffffffu, sum - mine, warp);
+  const int start = before + s.prefix[32 * warp + lane];
+  const int thread = __popc(__ballot_sync(0xffffffffu, start <= first)) - 1;
+  return make_int2(32 * warp + thread, __shfl_sync(0xffffffffu, start, thread));
 }
 
-__device__ __forceinline__ void next_batch(const PagedInt4& p, Walk& w, Batch& b, int lane) {
-  const int per_page = p.page_size / kInt4Tile;
-  int filled = 0, mine = -1, tokens = 0;
-  b.row = 0;
-  while (filled < 32 && w.left > 0 && w.row < p.batch * p.kv_heads) {
-    if (w.row - w.base >= 32) load_lengths(p, w, lane);
-    const int length = __shfl_sync(0xffffffffu, w.length, w.row - w.base);
-    const int tiles = (length + kInt4Tile - 1) / kInt4Tile;
-    const int n = min(min(32 - filled, tiles - w.tile), w.left);
-    if (lane >= filled && lane < filled + n) {
-      mine = w.tile + lane - filled;
-      tokens = length;
-      b.row = w.row;
-    }
-    filled += n, w.left -= n, w.tile += n;
-    if (w.tile == tiles) ++w.row, w.tile = 0;
+// Lengths of 32 rows, a lane each.
+struct Lengths {
+  int base, tokens;
+  const int* shared;  // the lengths of all rows in shared memory, if they are there
+  __device__ __forceinline__ void load(const PagedInt4& p, int row, int lane) {
+    base = row;
+    tokens = row + lane >= p.batch * p.kv_heads ? 0 : shared != nullptr ? shared[row + lane] : row_tokens_at(p, row + lane);
   }
-  b.tile = kBadTile;
-  b.meta = 0;
-  if (mine >= 0) {
-    const int h = b.row % p.kv_heads;
-    const int64_t page = page_id(p, b.row / p.kv_heads, h, mine / per_page);
-    if (page >= 0 && page < p.num_pages) {
-      b.tile = static_cast<uint32_t>((page * p.kv_heads + h) * per_page + mine % per_page);
-    } else {
-      atomicMax(p.status, kStatusBadPageId);
-    }
-    b.meta = min(tokens - mine * kInt4Tile, kInt4Tile) | (mine == 0 ? kRowStart : 0) | ((mine + 1) * kInt4Tile >= tokens ? kRowEnd : 0);
+  __device__ __forceinline__ int of(const PagedInt4& p, int row, int lane) {
+    if (row - base >= 32) load(p, row, lane);
+    return __shfl_sync(0xffffffffu, tokens, row - base);
   }
-}
+};
+
+// The next 32 units to request: lane i holds the two tiles of unit i, kNoTile for one behind the
+// row's end or in a page outside the pool.
+struct Requests {
+  Lengths lengths;
+  int row, unit;  // the next one
+  int left;
+  uint32_t tile[2];
+
+  __device__ __forceinline__ void refill(const PagedInt4& p, int lane) {
+    int filled = 0, mine = -1, mine_row = 0, mine_tokens = 0;
+    while (filled < 32 && left > 0 && row < p.batch * p.kv_heads) {
+      const int tokens = lengths.of(p, row, lane);
+      const int units = (tokens + kUnit - 1) / kUnit;
+      const int n = min(min(32 - filled, units - unit), left);
+      if (lane >= filled && lane < filled + n) mine = unit + lane - filled, mine_row = row, mine_tokens = tokens;
+      filled += n, left -= n, unit += n;
+      if (unit >= units) ++row, unit = 0;
+    }
+    tile[0] = tile[1] = kNoTile;
+    if (mine < 0) return;
+    const int2 at = row_place(p, mine_row);
+    const int first = 2 * mine, second = (first + 1) * kInt4Tile < mine_tokens ? first + 1 : first;
+    const int page0 = quotient(first, p.by_tiles), page1 = quotient(second, p.by_tiles);
+    const int64_t id0 = page_id(p, at.x, at.y, page0), id1 = page_id(p, at.x, at.y, page1);
+    const bool ok0 = id0 >= 0 && id0 < p.num_pages, ok1 = id1 >= 0 && id1 < p.num_pages;
+    if (!ok0 || !ok1) atomicMax(p.status, kStatusBadPageId);
+    if (ok0) tile[0] = (static_cast<uint32_t>(id0) * p.kv_heads + at.y - page0) * p.by_tiles.d + first;
+    if (ok1 && second != first) tile[1] = (static_cast<uint32_t>(id1) * p.kv_heads + at.y - page1) * p.by_tiles.d + second;
+  }
+};
+
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  using type = __half2;
+  static __device__ __forceinline__ __half2 of(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static __device__ __forceinline__ __nv_bfloat162 of(uint32_t x) { return *reinterpret_cast<__nv_bfloat162*>(&x); }
+};
 
 template <typename T, int D, int NT>
 struct Row {
@@ -181,26 +234,31 @@ struct Row {
   uint32_t qs[NT][2];         // and of the floors' product
   float c[NT][2];             // log2 units per unit of the products, heads 2t and 2t + 1 of an n-tile
   float o[NT][2 * W][4];
-  float z[NT][W][2];          // this lane's tokens' p * floor
+  uint64_t z[NT][W / 2][2];   // this lane's tokens' p * floor: pairs of groups, head 2t or 2t + 1
   float l[NT][2];             // and p
-  float m[NT][2];             // offset = m + e - 10
+  float off[NT][2];           // largest score so far (of the last raise) + e - 10
   int e;
 
   // Query rows as fp16 with the largest element in [2^9, 2^10): a power of two, so exact but for
   // elements 2^-20 below the largest.
-  __device__ __forceinline__ void start(const PagedInt4& p, int row, int group, int lane) {
-    const int b = row / p.kv_heads, h = row % p.kv_heads;
-    const int g = lane >> 2, t = lane & 3;
-    const T* src = static_cast<const T*>(p.q) + b * p.q_sb + static_cast<int64_t>(h) * group * p.q_sh;
+  static __device__ __forceinline__ void load(const PagedInt4& p, int row, int group, int lane, uint4 (&raw)[NT][W]) {
+    const int2 at = row_place(p, row);
+    const T* src = static_cast<const T*>(p.q) + at.x * p.q_sb + static_cast<int64_t>(at.y) * group * p.q_sh + 8 * (lane & 3);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int head = 8 * i + g;
-      uint4 raw[W];
+      const int head = 8 * i + (lane >> 2);
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        raw[w] = make_uint4(0, 0, 0, 0);
-        if (head < group) raw[w] = *reinterpret_cast<const uint4*>(src + head * p.q_sh + 32 * w + 8 * t);
+        raw[i][w] = make_uint4(0, 0, 0, 0);
+        if (head < group) raw[i][w] = *reinterpret_cast<const uint4*>(src + head * p.q_sh + 32 * w);
       }
+    }
+  }
+  __device__ __forceinline__ void start(const PagedInt4& p, const uint4 (&all)[NT][W], int lane) {
+    const int t = lane & 3;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const uint4(&raw)[W] = all[i];
       float top = 0.f;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
@@ -259,9 +317,9 @@ struct Row {
       c[i][1] = __shfl_sync(0xffffffffu, scale, 8 * t + 4);
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        l[i][y] = 0.f, m[i][y] = -INFINITY;
+        l[i][y] = 0.f, off[i][y] = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < W; ++w) z[i][w][y] = 0.f;
+        for (int w = 0; w < W / 2; ++w) z[i][w][y] = 0u;
       }
 #pragma unroll
       for (int w = 0; w < 2 * W; ++w) o[i][w][0] = o[i][w][1] = o[i][w][2] = o[i][w][3] = 0.f;
@@ -287,25 +345,43 @@ struct Row {
     }
   }
 
-  // Raise the offset to this tile's largest scores and steps.
-  __device__ __forceinline__ void raise(const float (&s)[NT][4], float magnitude) {
+  // exp2 arguments of the scores x, those behind the row's end -inf
+  __device__ __forceinline__ void arguments(const float (&x)[NT][8], float (&a)[NT][8], int left, int g) const {
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) magnitude = fmaxf(magnitude, __shfl_xor_sync(0xffffffffu, magnitude, off));
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[i][j] = fmaf(x[i][j], c[i][j & 1], -off[i][j & 1]);
+    }
+    if (__any_sync(0xffffffffu, left < kUnit)) {  // a vote: the compiler then knows the branch is the warp's
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[i][j] = g + 8 * (j >> 1) < left ? a[i][j] : -INFINITY;
+      }
+    }
+  }
+
+  // Raise the offset to this unit's largest scores and steps.
+  __device__ __forceinline__ void raise(const float (&x)[NT][8], float magnitude, int left, int g) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) magnitude = fmaxf(magnitude, __shfl_xor_sync(0xffffffffu, magnitude, d));
     const int above = max(-60, (__float_as_int(magnitude) >> 23) - 126);  // magnitude < 2^above
     const int next = max(e, min(above, 100));
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        float top = fmaxf(s[i][y], s[i][2 + y]);
+        float top = -INFINITY;
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        top = fmaxf(top, m[i][y]);
-        const float keep = fast_exp2((m[i][y] - top) + static_cast<float>(e - next));
-        m[i][y] = top;
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, g + 8 * j < left ? x[i][2 * j + y] * c[i][y] : -INFINITY);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float raised = fmaxf(top, off[i][y] - static_cast<float>(e - 10)) + static_cast<float>(next - 10);
+        const float keep = fast_exp2(off[i][y] - raised);
+        off[i][y] = raised;
         l[i][y] *= keep;
 #pragma unroll
-        for (int w = 0; w < W; ++w) z[i][w][y] *= keep;
+        for (int w = 0; w < W / 2; ++w) z[i][w][y] = mul32x2(z[i][w][y], pair32(keep, keep));
 #pragma unroll
         for (int w = 0; w < 2 * W; ++w) o[i][w][y] *= keep, o[i][w][2 + y] *= keep;
       }
@@ -313,114 +389,130 @@ struct Row {
     e = next;
   }
 
-  __device__ __forceinline__ void tile(const uint8_t* smem, int tokens, int lane) {
+  // Scores of one tile, in units of c: x[.][0..3] are (token g, heads 2t, 2t + 1), (token g + 8, ..).
+  __device__ __forceinline__ void scores(const uint8_t* smem, float (&x)[NT][8], int at, int lane) const {
     const int g = lane >> 2, t = lane & 3;
-    // scores
-    float s[NT][4];
-    {
-      float x[NT][4], y[NT][4];
-      uint32_t k0[W], k1[W], a0[W / 2], a1[W / 2];
-      unpack_words(smem + g * (D / 2) + t * 4 * W, k0);
-      unpack_words(smem + (g + 8) * (D / 2) + t * 4 * W, k1);
-      const uint8_t* params = smem + 16 * D;
-      unpack_params(params + g * 2 * W, a0);
-      unpack_params(params + (g + 8) * 2 * W, a1);
-      const int pair = W == 4 ? (t & 1) * 4 : 0;
-      const uint32_t f0 = *reinterpret_cast<const uint32_t*>(params + D + g * 2 * W + pair);
-      const uint32_t f1 = *reinterpret_cast<const uint32_t*>(params + D + (g + 8) * 2 * W + pair);
+    uint32_t k0[W], k1[W], a0[W / 2], a1[W / 2];
+    unpack_words(smem + g * (D / 2) + t * 4 * W, k0);
+    unpack_words(smem + (g + 8) * (D / 2) + t * 4 * W, k1);
+    const uint8_t* params = smem + 16 * D;
+    unpack_params(params + g * 2 * W, a0);
+    unpack_params(params + (g + 8) * 2 * W, a1);
+    const int pair = W == 4 ? (t & 1) * 4 : 0;
+    const uint32_t f0 = *reinterpret_cast<const uint32_t*>(params + D + g * 2 * W + pair);
+    const uint32_t f1 = *reinterpret_cast<const uint32_t*>(params + D + (g + 8) * 2 * W + pair);
+    float sum[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) sum[i][0] = sum[i][1] = sum[i][2] = sum[i][3] = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const uint32_t u0 = k0[w] >> 8, u1 = k1[w] >> 8;
+      const float2 step0 = unpack2<T>(a0[w / 2]), step1 = unpack2<T>(a1[w / 2]);
+      const float st0 = w % 2 ? step0.y : step0.x, st1 = w % 2 ? step1.y : step1.x;
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        y[i][0] = y[i][1] = y[i][2] = y[i][3] = 0.f;
-        mma_t<T>(y[i], f0, f1, f0, f1, qs[i][0], qs[i][1]);
-        x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_f16(d, k0[w] & 0x000f000fu, k1[w] & 0x000f000fu, k0[w] & 0x00f000f0u, k1[w] & 0x00f000f0u, q[i][2 * w][0], q[i][2 * w][1]);
+        mma_f16(d, u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, q[i][2 * w + 1][0], q[i][2 * w + 1][1]);
+        sum[i][0] = fmaf(st0, d[0], sum[i][0]), sum[i][1] = fmaf(st0, d[1], sum[i][1]);
+        sum[i][2] = fmaf(st1, d[2], sum[i][2]), sum[i][3] = fmaf(st1, d[3], sum[i][3]);
       }
+    }
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const uint32_t u0 = k0[w] >> 8, u1 = k1[w] >> 8;
-        const float2 step0 = unpack2<T>(a0[w / 2]), step1 = unpack2<T>(a1[w / 2]);
-        const float st0 = w % 2 ? step0.y : step0.x, st1 = w % 2 ? step1.y : step1.x;
+    for (int i = 0; i < NT; ++i) {
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+      mma_t<T>(y, f0, f1, f0, f1, qs[i][0], qs[i][1]);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_f16(d, k0[w] & 0x000f000fu, k1[w] & 0x000f000fu, k0[w] & 0x00f000f0u, k1[w] & 0x00f000f0u, q[i][2 * w][0], q[i][2 * w][1]);
-          mma_f16(d, u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, q[i][2 * w + 1][0], q[i][2 * w + 1][1]);
-          x[i][0] = fmaf(st0, d[0], x[i][0]), x[i][1] = fmaf(st0, d[1], x[i][1]);
-          x[i][2] = fmaf(st1, d[2], x[i][2]), x[i][3] = fmaf(st1, d[3], x[i][3]);
+      for (int j = 0; j < 4; ++j) x[i][at + j] = fmaf(sum[i][j], 16777216.f, y[j]);
+    }
+  }
+
+  // Two tiles, `left` tokens of the row from their first on.
+  __device__ __forceinline__ void unit(const uint8_t* smem, int left, int lane) {
+    using V2 = typename Pair<T>::type;
+    const int g = lane >> 2, t = lane & 3;
+    float x[NT][8];
+    scores(smem, x, 0, lane);
+    scores(smem + 20 * D, x, 4, lane);
+    // values' steps and floors; what lies behind the last token may be anything
+    uint32_t vc[4][W / 2], ve[4][W / 2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint8_t* params = smem + (k >> 1) * 20 * D + 18 * D + (g + 8 * (k & 1)) * 2 * W;
+      unpack_params(params, vc[k]);
+      unpack_params(params + D, ve[k]);
+    }
+    if (__any_sync(0xffffffffu, left < kUnit)) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int j = 0; j < W / 2; ++j) {
+          vc[k][j] = g + 8 * k < left ? vc[k][j] : 0u;
+          ve[k][j] = g + 8 * k < left ? ve[k][j] : 0u;
+        }
+      }
+    }
+    V2 steps = Pair<T>::of(vc[0][0]), floors = __habs2(Pair<T>::of(ve[0][0]));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int j = 0; j < W / 2; ++j) {
+        steps = __hmax2(steps, Pair<T>::of(vc[k][j]));
+        floors = __hmax2(floors, __habs2(Pair<T>::of(ve[k][j])));
+      }
+    }
+    const float magnitude = fmaxf(fmaxf(to_float(steps.x), to_float(steps.y)), 0.015625f * fmaxf(to_float(floors.x), to_float(floors.y)));
+    float a[NT][8];
+    arguments(x, a, left, g);
+    float top = a[0][0];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, a[i][j]);
+    }
+    if (__any_sync(0xffffffffu, (top > static_cast<float>(14 - e)) | (magnitude > pow2i(e)))) {
+      raise(x, magnitude, left, g);
+      arguments(x, a, left, g);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t v0[W], v1[W];
+      unpack_words(smem + k * 20 * D + 8 * D + t * D + g * 4 * W, v0);
+      unpack_words(smem + k * 20 * D + 8 * D + (t + 4) * D + g * 4 * W, v1);
+      uint32_t pb[NT][W][2];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        float pr[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pr[j] = fast_exp2(a[i][4 * k + j]);
+        l[i][0] += pr[0] + pr[2];
+        l[i][1] += pr[1] + pr[3];
+        uint64_t twice[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) twice[j] = pair32(pr[j], pr[j]);
+#pragma unroll
+        for (int w = 0; w < W / 2; ++w) {
+          const float2 s0 = unpack2<T>(vc[2 * k][w]), s1 = unpack2<T>(vc[2 * k + 1][w]);
+          const float2 f0 = unpack2<T>(ve[2 * k][w]), f1 = unpack2<T>(ve[2 * k + 1][w]);
+          const uint64_t c0 = pair32(s0.x, s0.y), c1 = pair32(s1.x, s1.y), e0 = pair32(f0.x, f0.y), e1 = pair32(f1.x, f1.y);
+          z[i][w][0] = fma32x2(twice[0], e0, fma32x2(twice[2], e1, z[i][w][0]));
+          z[i][w][1] = fma32x2(twice[1], e0, fma32x2(twice[3], e1, z[i][w][1]));
+          const float2 p0 = unpair32(mul32x2(twice[0], c0)), p1 = unpair32(mul32x2(twice[1], c0));
+          const float2 p2 = unpair32(mul32x2(twice[2], c1)), p3 = unpair32(mul32x2(twice[3], c1));
+          pb[i][2 * w][0] = transpose8(pack2<__half>(p0.x, p1.x));
+          pb[i][2 * w + 1][0] = transpose8(pack2<__half>(p0.y, p1.y));
+          pb[i][2 * w][1] = transpose8(pack2<__half>(p2.x, p3.x));
+          pb[i][2 * w + 1][1] = transpose8(pack2<__half>(p2.y, p3.y));
         }
       }
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = fmaf(x[i][j], 16777216.f, y[i][j]) * c[i][j & 1];
-      }
-    }
-    // values' steps and floors; what lies behind the last token may be anything
-    uint32_t c0[W / 2], c1[W / 2], e0[W / 2], e1[W / 2];
-    {
-      const uint8_t* params = smem + 18 * D;
-      unpack_params(params + g * 2 * W, c0);
-      unpack_params(params + (g + 8) * 2 * W, c1);
-      unpack_params(params + D + g * 2 * W, e0);
-      unpack_params(params + D + (g + 8) * 2 * W, e1);
-    }
-    if (tokens < kInt4Tile) {
-#pragma unroll
-      for (int j = 0; j < W / 2; ++j) {
-        if (g >= tokens) c0[j] = e0[j] = 0u;
-        if (g + 8 >= tokens) c1[j] = e1[j] = 0u;
-      }
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        if (g >= tokens) s[i][0] = s[i][1] = -INFINITY;
-        if (g + 8 >= tokens) s[i][2] = s[i][3] = -INFINITY;
-      }
-    }
-    float vc0[W], vc1[W], ve0[W], ve1[W];
-    float magnitude = 0.f;
-#pragma unroll
-    for (int j = 0; j < W / 2; ++j) {
-      const float2 w0 = unpack2<T>(c0[j]), w1 = unpack2<T>(c1[j]), w2 = unpack2<T>(e0[j]), w3 = unpack2<T>(e1[j]);
-      vc0[2 * j] = w0.x, vc0[2 * j + 1] = w0.y, vc1[2 * j] = w1.x, vc1[2 * j + 1] = w1.y;
-      ve0[2 * j] = w2.x, ve0[2 * j + 1] = w2.y, ve1[2 * j] = w3.x, ve1[2 * j + 1] = w3.y;
-    }
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      magnitude = fmaxf(magnitude, fmaxf(vc0[w], vc1[w]));
-      magnitude = fmaxf(magnitude, 0.015625f * fmaxf(fabsf(ve0[w]), fabsf(ve1[w])));
-    }
-    bool over = magnitude > pow2i(e);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) over = over || s[i][j] > m[i][j & 1] + 4.f;
-    }
-    if (__any_sync(0xffffffffu, over)) raise(s, magnitude);
-    uint32_t v0[W], v1[W];
-    unpack_words(smem + 8 * D + t * D + g * 4 * W, v0);
-    unpack_words(smem + 8 * D + (t + 4) * D + g * 4 * W, v1);
-    uint32_t pb[NT][W][2];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      float pr[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) pr[j] = fast_exp2(s[i][j] - (m[i][j & 1] + static_cast<float>(e - 10)));
-      l[i][0] += pr[0] + pr[2];
-      l[i][1] += pr[1] + pr[3];
-#pragma unroll
       for (int w = 0; w < W; ++w) {
-        z[i][w][0] = fmaf(pr[0], ve0[w], fmaf(pr[2], ve1[w], z[i][w][0]));
-        z[i][w][1] = fmaf(pr[1], ve0[w], fmaf(pr[3], ve1[w], z[i][w][1]));
-        pb[i][w][0] = transpose8(pack2<__half>(pr[0] * vc0[w], pr[1] * vc0[w]));
-        pb[i][w][1] = transpose8(pack2<__half>(pr[2] * vc1[w], pr[3] * vc1[w]));
-      }
-    }
+        const uint32_t u0 = v0[w] >> 8, u1 = v1[w] >> 8;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const uint32_t u0 = v0[w] >> 8, u1 = v1[w] >> 8;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        mma_f16(o[i][2 * w], v0[w] & 0x000f000fu, v0[w] & 0x00f000f0u, v1[w] & 0x000f000fu, v1[w] & 0x00f000f0u, pb[i][w][0], pb[i][w][1]);
-        mma_f16(o[i][2 * w + 1], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, pb[i][w][0], pb[i][w][1]);
+        for (int i = 0; i < NT; ++i) {
+          mma_f16(o[i][2 * w], v0[w] & 0x000f000fu, v0[w] & 0x00f000f0u, v1[w] & 0x000f000fu, v1[w] & 0x00f000f0u, pb[i][w][0], pb[i][w][1]);
+          mma_f16(o[i][2 * w + 1], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, pb[i][w][0], pb[i][w][1]);
+        }
       }
     }
   }
@@ -435,12 +527,14 @@ struct Row {
         for (int off = 4; off < 32; off <<= 1) l[i][y] += __shfl_xor_sync(0xffffffffu, l[i][y], off);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
+          const float2 both = unpair32(z[i][w / 2][y]);
+          float sum = w % 2 ? both.y : both.x;
 #pragma unroll
-          for (int off = 4; off < 32; off <<= 1) z[i][w][y] += __shfl_xor_sync(0xffffffffu, z[i][w][y], off);
+          for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            o[i][2 * w + k][y] = fmaf(o[i][2 * w + k][y], 16777216.f, z[i][w][y]);
-            o[i][2 * w + k][2 + y] = fmaf(o[i][2 * w + k][2 + y], 1048576.f, z[i][w][y]);
+            o[i][2 * w + k][y] = fmaf(o[i][2 * w + k][y], 16777216.f, sum);
+            o[i][2 * w + k][2 + y] = fmaf(o[i][2 * w + k][2 + y], 1048576.f, sum);
           }
         }
       }
@@ -448,7 +542,8 @@ struct Row {
   }
 
   __device__ __forceinline__ void write_out(const PagedInt4& p, int row, int group, int lane) const {
-    const int b = row / p.kv_heads, h = row % p.kv_heads, g = lane >> 2, t = lane & 3;
+    const int2 at = row_place(p, row);
+    const int b = at.x, h = at.y, g = lane >> 2, t = lane & 3;
     T* dst = static_cast<T*>(p.out) + b * p.o_sb + static_cast<int64_t>(h) * group * p.o_sh + 4 * g;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -483,31 +578,25 @@ struct Row {
         }
         if (g == 0) {
           *reinterpret_cast<float2*>(piece + S::kHeads * S::kStride + 2 * head) =
-              make_float2(m[i][y] + static_cast<float>(e - 10), l[i][y]);
+              make_float2(off[i][y], l[i][y]);
         }
       }
     }
   }
 };
 
-// Running sum of pieces of one (row, head); a lane holds D / 32 channels from channel
-// lane * D / 32.  A piece's offset is finite, or NaN where its scores are.
+// The channels of one (row, head) that a lane sums over pieces: D / 32 from channel lane * D / 32.
 template <int D>
 struct Merge {
   static constexpr int C = D / 32;
-  float o[C], offset, sum;
+  float o[C];
   __device__ __forceinline__ void clear() {
-    offset = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) o[c] = 0.f;
   }
-  __device__ __forceinline__ void add(const float (&x)[C], float off, float l) {
-    const float top = fmaxf(offset, off);
-    const float a = sum == 0.f ? 0.f : fast_exp2(offset - top), b = fast_exp2(off - top);
-    sum = sum * a + l * b;
+  __device__ __forceinline__ void add(const float (&x)[C], float weight) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) o[c] = o[c] * a + x[c] * b;
-    offset = top;
+    for (int c = 0; c < C; ++c) o[c] = fmaf(x[c], weight, o[c]);
   }
   static __device__ __forceinline__ void load(const float* at, float (&x)[C]) {
     if constexpr (C == 4) {
@@ -519,8 +608,9 @@ struct Merge {
     }
   }
   template <typename T>
-  __device__ __forceinline__ void write_out(const PagedInt4& p, int row, int group, int head, int lane) const {
-    const int b = row / p.kv_heads, h = row % p.kv_heads;
+  __device__ __forceinline__ void write_out(const PagedInt4& p, int row, int group, int head, int lane, float sum) const {
+    const int2 at = row_place(p, row);
+    const int b = at.x, h = at.y;
     T* dst = static_cast<T*>(p.out) + b * p.o_sb + (static_cast<int64_t>(h) * group + head) * p.o_sh + lane * C;
     const float inv = __fdividef(1.f, sum);
     if constexpr (C == 4) {
@@ -532,6 +622,17 @@ struct Merge {
     }
   }
 };
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+  return x;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
+}
 
 // Scratch: two pieces a CTA for the second kernel (the row it shares with the CTAs before it, the
 // row it starts and shares with those behind), one a warp for the row a warp shares with the warps
@@ -546,17 +647,16 @@ __host__ __device__ Scratch carve(void* workspace, int ctas) {
   Scratch s;
   s.cta_pieces = static_cast<float*>(workspace);
   s.warp_pieces = s.cta_pieces + static_cast<int64_t>(2 * ctas) * Shape<D, NT>::kPiece;
-  s.spans = reinterpret_cast<int2*>(s.warp_pieces + static_cast<int64_t>(kWarps * ctas) * Shape<D, NT>::kPiece);
+  s.spans = reinterpret_cast<int2*>(s.warp_pieces + static_cast<int64_t>(Shape<D, NT>::kWarps * ctas) * Shape<D, NT>::kPiece);
   return s;
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtasPerSm) int4_attention_kernel(const PagedInt4 p, int chunk) {
+__global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kernel(const PagedInt4 p, int chunk) {
   using S = Shape<D, NT>;
+  constexpr int kWarps = S::kWarps;
   extern __shared__ __align__(128) uint8_t s_ring[];
-  __shared__ __align__(8) uint64_t s_bar[kWarps][S::kStages];
-  __shared__ int64_t s_prefix[kThreads];
-  __shared__ int64_t s_warp[kWarps];
+  __shared__ Shares<kWarps> s_shares;
   __shared__ int s_row[2 * kWarps];    // rows of the pieces left to merge, warp by warp (first, last), -1: none
   __shared__ int s_flags[2 * kWarps];  // kRowStart / kRowEnd of those pieces
 
@@ -565,195 +665,231 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtasPerSm) int4_atten
   const int group = p.q_heads / p.kv_heads;
   const Scratch scratch = carve<D, NT>(p.workspace, ctas);
   uint8_t* ring = s_ring + warp * S::kRing;
-  const uint32_t ring_at = smem_u32(ring), bar_at = smem_u32(&s_bar[warp][0]);
-  if (lane < S::kStages) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar_at + 8 * lane));
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   if (threadIdx.x < 2 * kWarps) s_row[threadIdx.x] = -1;
   release_dependents();
   dependency_wait();
-  const Plan plan = make_plan(p, s_prefix, s_warp, chunk, ctas);
+  const Plan plan = make_plan(p, s_shares, chunk, ctas);
 
   // this warp's units
-  const int64_t cta_first = min(plan.share * cta, plan.units);
-  const int64_t cta_units = min(plan.share, plan.units - cta_first);
-  const int64_t first = cta_first + cta_units * warp / kWarps;
-  const int units = static_cast<int>(cta_first + cta_units * (warp + 1) / kWarps - first);
+  const int cta_first = static_cast<int>(min(static_cast<int64_t>(plan.share) * cta, static_cast<int64_t>(plan.units)));
+  const int cta_units = min(plan.share, plan.units - cta_first);
+  const int first = cta_first + static_cast<int>(static_cast<int64_t>(cta_units) * warp / kWarps);
+  const int units = cta_first + static_cast<int>(static_cast<int64_t>(cta_units) * (warp + 1) / kWarps) - first;
 
   if (units > 0) {
-    Walk walk;
+    Requests ahead;
     {
-      int lo = 0;
-#pragma unroll
-      for (int step = kThreads / 2; step > 0; step >>= 1) {
-        if (s_prefix[lo + step] <= first) lo += step;
-      }
-      walk.row = lo * chunk;
-      int64_t before = first - s_prefix[lo];
-      load_lengths(p, walk, lane);
+      const int2 found = find_rows(s_shares, first, lane);
+      ahead.row = found.x * chunk;
+      int before = first - found.y;
+      ahead.lengths.shared = chunk == 1 ? s_shares.tokens : nullptr;
+      ahead.lengths.load(p, ahead.row, lane);
       const int rows = p.batch * p.kv_heads;
-      while (walk.row < rows) {
-        if (walk.row - walk.base >= 32) load_lengths(p, walk, lane);
-        const int tiles = (__shfl_sync(0xffffffffu, walk.length, walk.row - walk.base) + kInt4Tile - 1) / kInt4Tile;
-        if (before < tiles) break;
-        before -= tiles;
-        ++walk.row;
+      while (ahead.row < rows) {
+        const int in_row = (ahead.lengths.of(p, ahead.row, lane) + kUnit - 1) / kUnit;
+        if (before < in_row) break;
+        before -= in_row;
+        ++ahead.row;
       }
-      walk.tile = static_cast<int>(before);
-      walk.left = units;
+      ahead.unit = before;
+      ahead.left = units;
     }
-    Batch now, next;
-    next_batch(p, walk, now, lane);
-    next.tile = kBadTile, next.meta = 0, next.row = 0;
-
-    auto request = [&](int unit, const Batch& b) {
-      const uint32_t tile = __shfl_sync(0xffffffffu, b.tile, unit & 31);
-      const int stage = unit % S::kStages;
-      if (tile != kBadTile) {
-        if (lane == 0) {
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_at + 8 * stage), "r"(S::kTileBytes) : "memory");
-          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                           ring_at + stage * S::kTileBytes),
-                       "l"(p.pool + static_cast<int64_t>(tile) * S::kTileBytes), "r"(S::kTileBytes), "r"(bar_at + 8 * stage)
-                       : "memory");
-        }
-      } else {  // a page outside the pool: zeros
-        for (int i = lane; i < S::kTileBytes / 16; i += 32) {
-          *reinterpret_cast<uint4*>(ring + stage * S::kTileBytes + 16 * i) = make_uint4(0, 0, 0, 0);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_at + 8 * stage) : "memory");
-      }
-    };
-    for (int u = 0; u < S::kStages && u < units; ++u) request(u, now);
-
+    Lengths lengths = ahead.lengths;
+    int id = ahead.row, in_row = ahead.unit;  // of the unit at hand
     Row<T, D, NT> row;
-    bool starts = false, in_row = false;
-    int pieces = 0;
-    for (int u = 0; u < units; ++u) {
-      if ((u & 31) == 0) {
-        if (u > 0) now = next;
-        if (walk.left > 0) next_batch(p, walk, next, lane);
-      }
-      const int meta = __shfl_sync(0xffffffffu, now.meta, u & 31);
-      const int id = __shfl_sync(0xffffffffu, now.row, u & 31);
-      if (!in_row) {
-        row.start(p, id, group, lane);
-        starts = (meta & kRowStart) != 0;
-        in_row = true;
-        if (starts && lane == 0) {
-          // the CTAs that hold the row: this one and those its last tile reaches
-          const int tiles = static_cast<int>((row_tokens(p, id / p.kv_heads, id % p.kv_heads) + kInt4Tile - 1) / kInt4Tile);
-          scratch.spans[id] = make_int2(cta, static_cast<int>((first + u + tiles - 1) / plan.share));
-        }
-      }
-      const int stage = u % S::kStages;
-      if (!wait_stage(bar_at + 8 * stage, (u / S::kStages) & 1) && lane == 0) atomicMax(p.status, kStatusPipelineTimeout);
-      row.tile(ring + stage * S::kTileBytes, meta & 31, lane);
-      __syncwarp();
-      const int ahead = u + S::kStages;
-      if (ahead < units) request(ahead, (ahead ^ u) < 32 ? now : next);
-      if ((meta & kRowEnd) || u == units - 1) {
-        const bool ends = (meta & kRowEnd) != 0;
-        row.finish();
-        if (starts && ends) {
-          row.write_out(p, id, group, lane);
-        } else {
-          const bool last = u == units - 1;
-          row.deposit(last ? reinterpret_cast<float*>(ring) : scratch.warp_pieces + static_cast<int64_t>(cta * kWarps + warp) * S::kPiece, lane);
-          if (lane == 0) {
-            s_row[2 * warp + (last ? 1 : 0)] = id;
-            s_flags[2 * warp + (last ? 1 : 0)] = (starts ? kRowStart : 0) | (ends ? kRowEnd : 0);
+    uint4 queries[NT][D / kInt4Group];
+    row.load(p, id, group, lane, queries);
+    ahead.refill(p, lane);
+
+    int wanted = 0;                                     // units requested
+    uint32_t request_at = smem_u32(ring) + 16 * lane;  // where this lane's part of the next goes
+    const uint32_t ring_end = request_at + S::kRing;
+    const uint8_t* pool = p.pool + 16 * lane;
+    // One group of copies a call, an empty one behind the last unit.
+    auto request = [&]() {
+      if (wanted < units) {
+        if ((wanted & 31) == 0 && wanted > 0) ahead.refill(p, lane);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t tile = __shfl_sync(0xffffffffu, ahead.tile[k], wanted & 31);
+          const bool real = tile != kNoTile;
+          const uint8_t* src = pool + (real ? static_cast<int64_t>(tile) * S::kTileBytes : 0);
+#pragma unroll
+          for (int n = 0; n < S::kTileBytes / 512; ++n) copy16(request_at + k * S::kTileBytes + 512 * n, src + 512 * n, real);
+          if (S::kTileBytes % 512 != 0 && lane < S::kTileBytes % 512 / 16) {
+            constexpr int kDone = S::kTileBytes / 512 * 512;
+            copy16(request_at + k * S::kTileBytes + kDone, src + kDone, real);
           }
         }
-        in_row = false;
-        ++pieces;
+        ++wanted;
+        request_at = request_at + S::kStageBytes == ring_end ? request_at + S::kStageBytes - S::kRing : request_at + S::kStageBytes;
       }
+      copies_close();
+    };
+#pragma unroll
+    for (int k = 0; k < S::kStages - 1; ++k) request();
+
+    int done = 0;
+    const uint8_t* at = ring;
+    while (done < units) {
+      int tokens = 0;
+      while (id < p.batch * p.kv_heads) {
+        tokens = lengths.of(p, id, lane);
+        if (in_row * kUnit < tokens) break;
+        ++id, in_row = 0;
+      }
+      const int in_all = (tokens + kUnit - 1) / kUnit;
+      const int n = max(1, min(in_all - in_row, units - done));  // lengths that change under a call must not hang it
+      if (done > 0) row.load(p, id, group, lane, queries);
+      row.start(p, queries, lane);
+      const bool starts = in_row == 0, ends = in_row + n >= in_all;
+      // the CTAs that hold the row: this one and those its last unit reaches
+      if (starts && lane == 0) scratch.spans[id] = make_int2(cta, (first + done + in_all - 1) / plan.share);
+      int left = tokens - in_row * kUnit;
+      for (int k = 0; k < n; ++k, left -= kUnit) {
+        copies_wait<S::kStages - 2>();
+        __syncwarp();  // this unit is here, and every lane is done with the one before
+        request();     // into that one's place
+        row.unit(at, left, lane);
+        at = at + S::kStageBytes == ring + S::kRing ? ring : at + S::kStageBytes;
+      }
+      done += n;
+      row.finish();
+      if (starts && ends) {
+        row.write_out(p, id, group, lane);
+      } else {
+        const bool last = done == units;
+        __syncwarp();
+        row.deposit(last ? reinterpret_cast<float*>(ring) : scratch.warp_pieces + static_cast<int64_t>(cta * kWarps + warp) * S::kPiece, lane);
+        if (lane == 0) {
+          s_row[2 * warp + (last ? 1 : 0)] = id;
+          s_flags[2 * warp + (last ? 1 : 0)] = (starts ? kRowStart : 0) | (ends ? kRowEnd : 0);
+        }
+      }
+      in_row += n;
     }
   }
   __syncthreads();
 
-  // Rows that several warps, or several CTAs, hold: a warp takes the heads with its number.
-  for (int i = 0; i < 2 * kWarps;) {
-    const int id = s_row[i];
-    if (id < 0) {
-      ++i;
-      continue;
-    }
-    int end = i, last = i;
-    for (; end < 2 * kWarps && (s_row[end] == id || s_row[end] < 0); ++end) last = s_row[end] == id ? end : last;
-    const bool starts = (s_flags[i] & kRowStart) != 0, ends = (s_flags[last] & kRowEnd) != 0;
+  // Rows that several warps, or several CTAs, hold: a warp takes the head with its number, a lane
+  // the offset and the sum of one piece.
+  const int my_row = lane < 2 * kWarps ? s_row[lane] : -1;
+  const int my_flags = my_row >= 0 ? s_flags[lane] : 0;
+  const float* warp_pieces = scratch.warp_pieces + static_cast<int64_t>(cta) * kWarps * S::kPiece;
+  auto piece_of = [&](int k) {
+    return (k & 1) ? reinterpret_cast<const float*>(s_ring + (k >> 1) * S::kRing) : warp_pieces + (k >> 1) * S::kPiece;
+  };
+  for (unsigned rest = __ballot_sync(0xffffffffu, my_row >= 0); rest != 0u;) {
+    const int i = __ffs(rest) - 1;
+    const int id = __shfl_sync(0xffffffffu, my_row, i);
+    const unsigned chain = __ballot_sync(0xffffffffu, my_row == id);
+    rest &= ~chain;
+    const bool starts = (__shfl_sync(0xffffffffu, my_flags, i) & kRowStart) != 0;
+    const bool ends = (__shfl_sync(0xffffffffu, my_flags, 31 - __clz(chain)) & kRowEnd) != 0;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int head = 8 * nt + warp;
+    for (int nt = 0; nt < (S::kHeads + kWarps - 1) / kWarps; ++nt) {
+      const int head = kWarps * nt + warp;  // eight warps and more: a head a warp, twice for 16 heads
       if (head >= group) break;
-      Merge<D> sum;
-      sum.clear();
-      for (int k = i; k <= last; ++k) {
-        if (s_row[k] < 0) continue;
-        const float* piece = (k & 1) ? reinterpret_cast<const float*>(s_ring + (k >> 1) * S::kRing)
-                                     : scratch.warp_pieces + static_cast<int64_t>(cta * kWarps + (k >> 1)) * S::kPiece;
-        float x[Merge<D>::C];
-        Merge<D>::load(piece + head * S::kStride + lane * Merge<D>::C, x);
-        const float2 ml = *reinterpret_cast<const float2*>(piece + S::kHeads * S::kStride + 2 * head);
-        sum.add(x, ml.x, ml.y);
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (my_row == id) ml = *reinterpret_cast<const float2*>(piece_of(lane) + S::kHeads * S::kStride + 2 * head);
+      const float top = warp_max(ml.x);
+      const float weight = my_row == id ? fast_exp2(ml.x - top) : 0.f;
+      const float sum = warp_sum(ml.y * weight);
+      Merge<D> merge;
+      merge.clear();
+      for (unsigned left = chain; left != 0u;) {
+        float x[4][Merge<D>::C], scale[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {  // four pieces in flight; the last one again, weightless, where fewer are left
+          const int k = left != 0u ? __ffs(left) - 1 : i;
+          scale[n] = __shfl_sync(0xffffffffu, weight, k);
+          if (left == 0u) scale[n] = 0.f;
+          left &= left - 1;
+          Merge<D>::load(piece_of(k) + head * S::kStride + lane * Merge<D>::C, x[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) merge.add(x[n], scale[n]);
       }
       if (starts && ends) {
-        sum.template write_out<T>(p, id, group, head, lane);
+        merge.template write_out<T>(p, id, group, head, lane, sum);
       } else {
         float* piece = scratch.cta_pieces + static_cast<int64_t>(2 * cta + (starts ? 1 : 0)) * S::kPiece;
 #pragma unroll
-        for (int c = 0; c < Merge<D>::C; ++c) piece[head * S::kStride + lane * Merge<D>::C + c] = sum.o[c];
-        if (lane == 0) *reinterpret_cast<float2*>(piece + S::kHeads * S::kStride + 2 * head) = make_float2(sum.offset, sum.sum);
+        for (int c = 0; c < Merge<D>::C; ++c) piece[head * S::kStride + lane * Merge<D>::C + c] = merge.o[c];
+        if (lane == 0) *reinterpret_cast<float2*>(piece + S::kHeads * S::kStride + 2 * head) = make_float2(top, sum);
       }
     }
-    i = end;
   }
 }
 
 // Rows that span CTAs, and zeros for rows without tokens: one CTA of four warps a (row, head),
 // the pieces dealt out to the warps in turn.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128) int4_combine_kernel(const PagedInt4 p, int ctas) {
+__global__ void __launch_bounds__(128) int4_combine_kernel(const PagedInt4 p, int ctas, Divisor by_group) {
   using S = Shape<D, NT>;
   constexpr int C = Merge<D>::C;
   __shared__ float s_o[4][D];
-  __shared__ float2 s_ml[4];
+  __shared__ float s_top[4], s_sum[4];
   release_dependents();
   dependency_wait();
-  const int group = p.q_heads / p.kv_heads;
-  const int row = blockIdx.x / group, head = blockIdx.x % group;
+  const int group = by_group.d;
+  const int row = quotient(blockIdx.x, by_group), head = blockIdx.x - row * group;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = row / p.kv_heads, h = row % p.kv_heads;
-  if (row_tokens(p, b, h) == 0) {
-    T* dst = static_cast<T*>(p.out) + b * p.o_sb + (static_cast<int64_t>(h) * group + head) * p.o_sh;
+  const Scratch scratch = carve<D, NT>(p.workspace, ctas);
+  const int2 span = scratch.spans[row];  // unwritten, and not used, for a row without tokens
+  if (row_tokens_at(p, row) == 0) {
+    const int2 at = row_place(p, row);
+    T* dst = static_cast<T*>(p.out) + at.x * p.o_sb + (static_cast<int64_t>(at.y) * group + head) * p.o_sh;
     for (int d = threadIdx.x; d < D; d += 128) dst[d] = from_float<T>(0.f);
     return;
   }
-  const Scratch scratch = carve<D, NT>(p.workspace, ctas);
-  const int2 span = scratch.spans[row];
   if (span.x == span.y) return;
-  Merge<D> sum;
-  sum.clear();
-#pragma unroll 4
-  for (int c = span.x + warp; c <= span.y; c += 4) {
-    const float* piece = scratch.cta_pieces + static_cast<int64_t>(2 * c + (c == span.x ? 1 : 0)) * S::kPiece;
-    float x[C];
-    Merge<D>::load(piece + head * S::kStride + lane * C, x);
-    const float2 ml = *reinterpret_cast<const float2*>(piece + S::kHeads * S::kStride + 2 * head);
-    sum.add(x, ml.x, ml.y);
+  auto piece_of = [&](int c) { return scratch.cta_pieces + static_cast<int64_t>(2 * c + (c == span.x ? 1 : 0)) * S::kPiece; };
+  // offset and sum of every piece, a lane each, 128 at a time; every warp sees all of them
+  float top = -INFINITY, sum = 0.f;
+  Merge<D> merge;
+  merge.clear();
+  for (int first = span.x; first <= span.y; first += 128) {
+    float2 ml = make_float2(-INFINITY, 0.f);
+    const int mine = first + 4 * lane + warp;  // a warp's pieces are every fourth
+    if (mine <= span.y) ml = *reinterpret_cast<const float2*>(piece_of(mine) + S::kHeads * S::kStride + 2 * head);
+    const float now = fmaxf(top, warp_max(ml.x));
+    const float keep = sum == 0.f ? 0.f : fast_exp2(top - now);
+    const float weight = mine <= span.y ? fast_exp2(ml.x - now) : 0.f;
+    top = now;
+    sum = sum * keep + warp_sum(ml.y * weight);
+#pragma unroll
+    for (int c = 0; c < C; ++c) merge.o[c] *= keep;
+    const int n = min(32, (span.y - first - warp + 4) / 4);  // pieces of this warp in this turn
+    for (int k = 0; k < n; k += 4) {
+      float x[4][C];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) Merge<D>::load(piece_of(first + 4 * min(k + y, n - 1) + warp) + head * S::kStride + lane * C, x[y]);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float scale = __shfl_sync(0xffffffffu, weight, (k + y) & 31);
+        merge.add(x[y], k + y < n ? scale : 0.f);
+      }
+    }
   }
 #pragma unroll
-  for (int c = 0; c < C; ++c) s_o[warp][lane * C + c] = sum.o[c];
-  if (lane == 0) s_ml[warp] = make_float2(sum.offset, sum.sum);
+  for (int c = 0; c < C; ++c) s_o[warp][lane * C + c] = merge.o[c];
+  if (lane == 0) s_top[warp] = top, s_sum[warp] = sum;
   __syncthreads();
   if (warp != 0) return;
-  for (int w = 1; w < 4 && span.x + w <= span.y; ++w) {
+  const int warps = min(4, span.y - span.x + 1);
+  float all = s_top[0];
+  for (int w = 1; w < warps; ++w) all = fmaxf(all, s_top[w]);
+  sum = 0.f;
+  merge.clear();
+  for (int w = 0; w < warps; ++w) {
+    const float weight = fast_exp2(s_top[w] - all);
     float x[C];
     Merge<D>::load(&s_o[w][lane * C], x);
-    sum.add(x, s_ml[w].x, s_ml[w].y);
+    merge.add(x, weight);
+    sum = fmaf(s_sum[w], weight, sum);
   }
-  sum.template write_out<T>(p, row, group, head, lane);
+  merge.template write_out<T>(p, row, group, head, lane, sum);
 }
 
 int sm_count() {
@@ -768,7 +904,7 @@ int sm_count() {
 
 template <int D, int NT>
 int64_t scratch_bytes(int64_t rows, int ctas) {
-  const int64_t pieces = static_cast<int64_t>(2 + kWarps) * ctas * Shape<D, NT>::kPiece * 4;
+  const int64_t pieces = static_cast<int64_t>(2 + Shape<D, NT>::kWarps) * ctas * Shape<D, NT>::kPiece * 4;
   return (pieces + rows * 8 + 15) / 16 * 16;
 }
 
@@ -776,7 +912,7 @@ template <typename T, int D, int NT>
 int launch(const PagedInt4& p, cudaStream_t stream) {
   using S = Shape<D, NT>;
   const int64_t rows = static_cast<int64_t>(p.batch) * p.kv_heads;
-  const int ctas = sm_count() * S::kCtasPerSm;
+  const int ctas = sm_count();
   const int64_t need = scratch_bytes<D, NT>(rows, ctas);
   QF_REQUIRE(p.workspace != nullptr && p.workspace_bytes >= need, "the workspace holds %lld bytes, %lld are needed",
              static_cast<long long>(p.workspace_bytes), static_cast<long long>(need));
@@ -788,10 +924,10 @@ int launch(const PagedInt4& p, cudaStream_t stream) {
     QF_CUDA(cudaFuncSetAttribute(int4_attention_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     ready = device;
   }
-  const int chunk = static_cast<int>((rows + kThreads - 1) / kThreads);
-  QF_CUDA(launch_chained(int4_attention_kernel<T, D, NT>, dim3(ctas), dim3(kThreads), static_cast<size_t>(S::kSmem), stream, p, chunk));
+  const int chunk = static_cast<int>((rows + S::kThreads - 1) / S::kThreads);
+  QF_CUDA(launch_chained(int4_attention_kernel<T, D, NT>, dim3(ctas), dim3(S::kThreads), static_cast<size_t>(S::kSmem), stream, p, chunk));
   QF_CUDA(launch_chained(int4_combine_kernel<T, D, NT>, dim3(static_cast<unsigned>(rows * (p.q_heads / p.kv_heads))), dim3(128),
-                         static_cast<size_t>(0), stream, p, ctas));
+                         static_cast<size_t>(0), stream, p, ctas, make_divisor(p.q_heads / p.kv_heads)));
   QF_CUDA(cudaGetLastError());
   return QF_OK;
 }
@@ -810,9 +946,9 @@ int64_t int4_attention_bytes(const PagedInt4& p, int head_dim) {
   const bool two = p.q_heads / p.kv_heads > 8;
   const int sms = sm_count();
   if (head_dim == 128) {
-    return two ? scratch_bytes<128, 2>(rows, sms * Shape<128, 2>::kCtasPerSm) : scratch_bytes<128, 1>(rows, sms * Shape<128, 1>::kCtasPerSm);
+    return two ? scratch_bytes<128, 2>(rows, sms) : scratch_bytes<128, 1>(rows, sms);
   }
-  return two ? scratch_bytes<64, 2>(rows, sms * Shape<64, 2>::kCtasPerSm) : scratch_bytes<64, 1>(rows, sms * Shape<64, 1>::kCtasPerSm);
+  return two ? scratch_bytes<64, 2>(rows, sms) : scratch_bytes<64, 1>(rows, sms);
 }
 
 int launch_int4_attention(const PagedInt4& p, int head_dim, int dtype, cudaStream_t stream) {

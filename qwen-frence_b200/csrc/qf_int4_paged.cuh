@@ -26,6 +26,7 @@ struct PagedInt4 {
   int batch, q_heads, kv_heads, page_size;
   int table_dtype, lens_dtype;
   int new_tokens, take;
+  Divisor by_heads, by_page, by_tiles;  // kv_heads, page_size, tiles of a page
 };
 
 enum : int { kNeedsQuery = 1, kNeedsPool = 2, kNeedsOut = 4, kNeedsBounds = 8, kNeedsSelection = 16 };
@@ -33,6 +34,12 @@ enum : int { kNeedsQuery = 1, kNeedsPool = 2, kNeedsOut = 4, kNeedsBounds = 8, k
 int fill_paged_int4(const qf_paged_int4_args* args, int needs, PagedInt4* p);
 int64_t int4_attention_bytes(const PagedInt4& p, int head_dim);  // scratch of launch_int4_attention
 int launch_int4_attention(const PagedInt4& p, int head_dim, int dtype, cudaStream_t stream);
+
+// (sequence, KV head) of a row.
+__device__ __forceinline__ int2 row_place(const PagedInt4& p, int row) {
+  const int b = quotient(row, p.by_heads);
+  return make_int2(b, row - b * p.kv_heads);
+}
 
 // Tokens of row (b, h): never negative, never more than its table row can hold.
 __device__ __forceinline__ int64_t row_tokens(const PagedInt4& p, int b, int h) {

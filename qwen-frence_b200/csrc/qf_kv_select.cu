@@ -19,8 +19,10 @@ int fill_paged_int4(const qf_paged_int4_args* a, int needs, PagedInt4* p) {
   QF_REQUIRE(a->num_pages >= 0 && a->num_pages < (1LL << 31) && a->table_width >= 0, "invalid pool or table size");
   // tiles of the pool are counted in 32 bits
   QF_REQUIRE(a->num_pages <= 0xfffffffeLL / a->kv_heads / (a->page_size / kInt4Tile), "invalid pool or table size");
-  // tokens of a row are counted in 32 bits
-  QF_REQUIRE(a->table_width <= ((1LL << 31) - 1) / a->page_size, "a block table row holds 2^31 tokens or more");
+  // tokens of a row, and tiles of all rows, are counted in 31 bits
+  QF_REQUIRE(a->table_width < (1LL << 30) / a->page_size, "a block table row holds 2^30 tokens or more");
+  QF_REQUIRE(static_cast<int64_t>(a->batch) * a->kv_heads * a->table_width < (1LL << 30) / (a->page_size / kInt4Tile),
+             "the block tables of a call hold 2^30 tiles of 16 tokens or more");
   if (needs & kNeedsQuery) {
     QF_REQUIRE(a->q_heads >= 1 && a->q_heads % a->kv_heads == 0, "query heads must be divisible by KV heads");
     QF_REQUIRE(a->q_heads / a->kv_heads <= 16, "at most 16 query heads share a KV head");
@@ -59,6 +61,8 @@ int fill_paged_int4(const qf_paged_int4_args* a, int needs, PagedInt4* p) {
   r.batch = a->batch, r.q_heads = a->q_heads, r.kv_heads = a->kv_heads, r.page_size = a->page_size;
   r.table_dtype = a->table_dtype, r.lens_dtype = a->lens_dtype;
   r.new_tokens = a->new_tokens, r.take = a->take;
+  r.by_heads = make_divisor(a->kv_heads), r.by_page = make_divisor(a->page_size);
+  r.by_tiles = make_divisor(a->page_size / kInt4Tile);
   if (a->batch > 0) {
     r.status = device_status_word();
     QF_REQUIRE(r.status != nullptr, "no device status word");
@@ -70,73 +74,86 @@ int fill_paged_int4(const qf_paged_int4_args* a, int needs, PagedInt4* p) {
 namespace {
 
 // The extremes of a page keep a NaN: a page that holds one must not look harmless.
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
-// One warp a (sequence, page, KV head).  A lane reads one word (eight channels) of a token's
-// codes, so 32 / (D / 8) tokens at a time; rounding to T is monotone and comes once, at the end.
+// One warp a (sequence, page, KV head), a lane eight channels of 16 / (32 / (D / 8)) tokens of
+// a tile: all the loads of a tile are in flight together.  Two tokens a step of the three-operand
+// minimum and maximum; rounding to T is monotone and comes once, at the end.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) key_bounds_kernel(const PagedInt4 p, int pages_each) {
-  constexpr int W = D / kInt4Group, kWords = D / 8, kTokens = 32 / kWords;
+__global__ void __launch_bounds__(128) key_bounds_kernel(const PagedInt4 p, const Divisor by_each) {
+  constexpr int W = D / kInt4Group, kWords = D / 8, kStep = 32 / kWords, kTokens = kInt4Tile / kStep;
   release_dependents();
   dependency_wait();
   const int lane = threadIdx.x % 32;
-  const int64_t unit = blockIdx.x * static_cast<int64_t>(blockDim.x / 32) + threadIdx.x / 32;
-  const int h = static_cast<int>(unit % p.kv_heads);
-  const int64_t rest = unit / p.kv_heads;
-  const int i = static_cast<int>(rest % pages_each);
-  const int64_t b = rest / pages_each;
-  if (b >= p.batch) return;
-  const int64_t tokens = row_tokens(p, static_cast<int>(b), 0);
-  const int64_t before = tokens > p.new_tokens ? tokens - p.new_tokens : 0;
-  const int64_t n = before / p.page_size + i;
-  if (n * p.page_size >= tokens) return;
-  const int64_t page = page_id(p, static_cast<int>(b), 0, n);
+  const uint32_t unit = blockIdx.x * 4 + threadIdx.x / 32;
+  const uint32_t row = quotient(unit, by_each);
+  const int2 at = row_place(p, row);
+  const int i = unit - row * by_each.d, h = at.y;
+  if (at.x >= p.batch) return;
+  const int tokens = static_cast<int>(row_tokens(p, at.x, 0));
+  const int before = tokens > p.new_tokens ? tokens - p.new_tokens : 0;
+  const int n = quotient(before, p.by_page) + i;
+  const int left = tokens - n * p.page_size;
+  if (n >= p.table_width || left <= 0) return;
+  const int64_t page = page_id(p, at.x, 0, n);
   if (page < 0 || page >= p.num_pages) {
     if (lane == 0) atomicMax(p.status, kStatusBadPageId);
     return;
   }
-  const int64_t left = tokens - n * p.page_size;
-  const int live = left < p.page_size ? static_cast<int>(left) : p.page_size;
-  const int word = lane % kWords, t = word / W, w = word % W;
+  const int live = min(left, p.page_size);
+  const int word = lane % kWords, t = word / W, w = word % W, first = lane / kWords;
   float low[8], high[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) low[j] = INFINITY, high[j] = -INFINITY;
-  for (int token = lane / kWords; token < live; token += kTokens) {
-    const uint8_t* tile = p.pool + ((page * p.kv_heads + h) * (p.page_size / kInt4Tile) + token / kInt4Tile) * int4_tile_bytes(D);
-    const int r = token % kInt4Tile;
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(tile + r * (D / 2) + 4 * word);
-    const T* params = reinterpret_cast<const T*>(tile + 16 * D) + r * W + w;
-    const float step = to_float(params[0]), floor = to_float(params[D / 2]);
+  const uint8_t* tile = p.pool + (page * p.kv_heads + h) * (p.page_size / kInt4Tile) * int4_tile_bytes(D);
+  for (int begin = 0; begin < live; begin += kInt4Tile, tile += int4_tile_bytes(D)) {
+    uint32_t codes[kTokens];
+    T steps[kTokens], floors[kTokens];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = int4_value((codes >> (4 * j)) & 15u, step, floor);
-      low[j] = min_nan(low[j], x), high[j] = max_nan(high[j], x);
+    for (int k = 0; k < kTokens; ++k) {
+      // behind the last token: the first one of the tile again, which every tile here has
+      const int r = begin + first + kStep * k < live ? first + kStep * k : 0;
+      codes[k] = *reinterpret_cast<const uint32_t*>(tile + r * (D / 2) + 4 * word);
+      const T* params = reinterpret_cast<const T*>(tile + 16 * D) + r * W + w;
+      steps[k] = params[0], floors[k] = params[D / 2];
+    }
+#pragma unroll
+    for (int k = 0; k < kTokens; k += 2) {
+      float x[8], y[8];
+      int4_values(codes[k], to_float(steps[k]), to_float(floors[k]), x);
+      int4_values(codes[k + 1], to_float(steps[k + 1]), to_float(floors[k + 1]), y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) low[j] = min_nan(low[j], x[j], y[j]), high[j] = max_nan(high[j], x[j], y[j]);
     }
   }
 #pragma unroll
   for (int off = kWords; off < 32; off <<= 1) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      low[j] = min_nan(low[j], __shfl_xor_sync(0xffffffffu, low[j], off));
-      high[j] = max_nan(high[j], __shfl_xor_sync(0xffffffffu, high[j], off));
+      const float a = __shfl_xor_sync(0xffffffffu, low[j], off), z = __shfl_xor_sync(0xffffffffu, high[j], off);
+      low[j] = min_nan(low[j], a, a), high[j] = max_nan(high[j], z, z);
     }
   }
   if (lane < kWords) {
     T* dst = static_cast<T*>(p.bounds) + (page * p.kv_heads + h) * 2 * D + 32 * w + 8 * t;
-    uint4 a, z;
-    a.x = pack2<T>(low[0], low[1]), a.y = pack2<T>(low[2], low[3]), a.z = pack2<T>(low[4], low[5]), a.w = pack2<T>(low[6], low[7]);
-    z.x = pack2<T>(high[0], high[1]), z.y = pack2<T>(high[2], high[3]), z.z = pack2<T>(high[4], high[5]), z.w = pack2<T>(high[6], high[7]);
-    *reinterpret_cast<uint4*>(dst) = a;
-    *reinterpret_cast<uint4*>(dst + D) = z;
+    *reinterpret_cast<uint4*>(dst) =
+        make_uint4(pack2<T>(low[0], low[1]), pack2<T>(low[2], low[3]), pack2<T>(low[4], low[5]), pack2<T>(low[6], low[7]));
+    *reinterpret_cast<uint4*>(dst + D) =
+        make_uint4(pack2<T>(high[0], high[1]), pack2<T>(high[2], high[3]), pack2<T>(high[4], high[5]), pack2<T>(high[6], high[7]));
   }
 }
 
@@ -147,116 +164,174 @@ __device__ __forceinline__ uint32_t score_key(float s) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// keys[row][n], row = b * kv_heads + h: D / 8 lanes a page, eight channels each.
+// keys[row][n], row = b * kv_heads + h: D / 8 lanes a page, eight channels each, two pages a lane
+// in flight; the row's queries are held as floats in shared memory.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) page_score_kernel(const PagedInt4 p, uint32_t* keys) {
-  constexpr int kLanes = D / 8, kPages = 32 / kLanes;
+  constexpr int kLanes = D / 8, kPages = 32 / kLanes, kMaxGroup = 16;
+  __shared__ __align__(16) float s_q[kMaxGroup][D];
   release_dependents();
   dependency_wait();
-  const int row = blockIdx.y, b = row / p.kv_heads, h = row % p.kv_heads;
+  const int row = blockIdx.y;
+  const int2 at = row_place(p, row);
+  const int b = at.x, h = at.y;
   const int lane = threadIdx.x % 32, l = lane % kLanes;
-  const int64_t tokens = row_tokens(p, b, 0);
-  const int count = static_cast<int>((tokens + p.page_size - 1) / p.page_size);
-  if (count <= p.take) return;  // every page is taken
+  const int tokens = static_cast<int>(row_tokens(p, b, 0));
+  const int count = quotient(tokens + p.page_size - 1, p.by_page);
+  const int warp_first = (blockIdx.x * 8 + threadIdx.x / 32) * 2 * kPages;
+  if (count <= p.take || blockIdx.x * 16 * kPages >= count - 1) return;  // every page is taken, or none is left
   const int group = p.q_heads / p.kv_heads;
-  const int step = gridDim.x * (blockDim.x / 32) * kPages;
-  for (int first = (blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) * kPages; first < count - 1; first += step) {
-    const int n = first + lane / kLanes;
-    const int64_t page = n < count - 1 ? page_id(p, b, 0, n) : 0;
-    const bool ok = n < count - 1 && page >= 0 && page < p.num_pages;
-    if (!ok && n < count - 1 && l == 0) atomicMax(p.status, kStatusBadPageId);
-    uint4 low = make_uint4(0, 0, 0, 0), high = low;
-    if (ok) {
-      const T* src = static_cast<const T*>(p.bounds) + (page * p.kv_heads + h) * 2 * D + 8 * l;
-      low = *reinterpret_cast<const uint4*>(src), high = *reinterpret_cast<const uint4*>(src + D);
-    }
-    float best = -INFINITY;
-    for (int g = 0; g < group; ++g) {
-      const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_sb + (h * group + g) * p.q_sh + 8 * l);
-      float sum[4];
+  for (int i = threadIdx.x; i < group * (D / 8); i += 256) {
+    const int g = i / (D / 8), d = i % (D / 8) * 8;
+    const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_sb + static_cast<int64_t>(h * group + g) * p.q_sh + d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(&s_q[g][d + 2 * j]) = unpack2<T>((&raw.x)[j]);
+  }
+  __syncthreads();
+  const int step = gridDim.x * 16 * kPages;
+  for (int first = warp_first; first < count - 1; first += step) {
+    float low[2][8], high[2][8];
+    bool ok[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int n = first + k * kPages + lane / kLanes;
+      const int64_t page = n < count - 1 ? page_id(p, b, 0, n) : -1;
+      ok[k] = page >= 0 && page < p.num_pages;
+      if (!ok[k] && n < count - 1 && l == 0) atomicMax(p.status, kStatusBadPageId);
+      uint4 a = make_uint4(0, 0, 0, 0), z = a;
+      if (ok[k]) {
+        const T* src = static_cast<const T*>(p.bounds) + (page * p.kv_heads + h) * 2 * D + 8 * l;
+        a = *reinterpret_cast<const uint4*>(src), z = *reinterpret_cast<const uint4*>(src + D);
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 x = unpack2<T>((&q.x)[j]), lo = unpack2<T>((&low.x)[j]), hi = unpack2<T>((&high.x)[j]);
-        sum[j] = __fadd_rn(max_nan(__fmul_rn(x.x, lo.x), __fmul_rn(x.x, hi.x)), max_nan(__fmul_rn(x.y, lo.y), __fmul_rn(x.y, hi.y)));
+        const float2 lo = unpack2<T>((&a.x)[j]), hi = unpack2<T>((&z.x)[j]);
+        low[k][2 * j] = lo.x, low[k][2 * j + 1] = lo.y, high[k][2 * j] = hi.x, high[k][2 * j + 1] = hi.y;
       }
-      float s = __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3]));
-#pragma unroll
-      for (int off = 1; off < kLanes; off <<= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, off));
-      best = max_nan(best, s);
     }
-    if (l == 0 && n < count - 1) keys[static_cast<int64_t>(row) * p.table_width + n] = ok ? score_key(best) : 0u;
+    float best[2] = {-INFINITY, -INFINITY};
+    for (int g = 0; g < group; ++g) {
+      float q[8];
+      *reinterpret_cast<float4*>(q) = *reinterpret_cast<const float4*>(&s_q[g][8 * l]);
+      *reinterpret_cast<float4*>(q + 4) = *reinterpret_cast<const float4*>(&s_q[g][8 * l + 4]);
+      float s[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float term[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) term[j] = max_nan(__fmul_rn(q[j], low[k][j]), __fmul_rn(q[j], high[k][j]));
+        s[k] = __fadd_rn(__fadd_rn(__fadd_rn(term[0], term[1]), __fadd_rn(term[2], term[3])),
+                         __fadd_rn(__fadd_rn(term[4], term[5]), __fadd_rn(term[6], term[7])));
+      }
+#pragma unroll
+      for (int off = 1; off < kLanes; off <<= 1) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) s[k] = __fadd_rn(s[k], __shfl_xor_sync(0xffffffffu, s[k], off));
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) best[k] = max_nan(best[k], s[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int n = first + k * kPages + lane / kLanes;
+      if (l == 0 && n < count - 1) keys[static_cast<int64_t>(row) * p.table_width + n] = ok[k] ? score_key(best[k]) : 0u;
+    }
   }
 }
 
-// One CTA a row.  The take - 1 largest keys of the pages before the newest: their smallest key
-// by radix, eight bits a pass, then the pages in order, those that tie with it as long as there
-// is room.
-__global__ void __launch_bounds__(1024) page_pick_kernel(const PagedInt4 p, const uint32_t* keys) {
-  __shared__ int s_count[256];
-  __shared__ int s_warp[2][32];
-  __shared__ uint32_t s_key;
-  __shared__ int s_left;
+constexpr int kPickThreads = 512;
+
+// Sums of three counts over the CTA.  `phase` alternates two buffers, so one barrier is enough.
+__device__ __forceinline__ int3 cta_sums(int a, int b, int c, int (*s_sum)[3][kPickThreads / 32], int phase) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  a = __reduce_add_sync(0xffffffffu, a), b = __reduce_add_sync(0xffffffffu, b), c = __reduce_add_sync(0xffffffffu, c);
+  if (lane == 0) s_sum[phase][0][warp] = a, s_sum[phase][1][warp] = b, s_sum[phase][2][warp] = c;
+  __syncthreads();
+  const bool on = lane < kPickThreads / 32;
+  a = on ? s_sum[phase][0][lane] : 0, b = on ? s_sum[phase][1][lane] : 0, c = on ? s_sum[phase][2][lane] : 0;
+  return make_int3(__reduce_add_sync(0xffffffffu, a), __reduce_add_sync(0xffffffffu, b), __reduce_add_sync(0xffffffffu, c));
+}
+
+// One CTA a row.  The take - 1 largest keys of the pages before the newest: the smallest of them
+// two bits at a time, by counting the keys at or above three candidates (equal keys cost what
+// different ones do), then the pages in order, those that tie with it as long as there is room.
+// A thread holds a run of kHeld neighbouring keys in registers; longer rows are read again from
+// the second level cache every time.
+template <int kHeld>
+__global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const PagedInt4 p, const uint32_t* keys) {
+  __shared__ int s_sum[2][3][kPickThreads / 32];
+  __shared__ int2 s_scan[kPickThreads / 32];
   release_dependents();
   dependency_wait();
-  const int row = blockIdx.x, b = row / p.kv_heads, h = row % p.kv_heads;
+  const int row = blockIdx.x;
+  const int2 at = row_place(p, row);
+  const int b = at.x;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const int64_t tokens = row_tokens(p, b, 0);
-  const int count = static_cast<int>((tokens + p.page_size - 1) / p.page_size);
+  const int tokens = static_cast<int>(row_tokens(p, b, 0));
+  const int count = quotient(tokens + p.page_size - 1, p.by_page);
   int32_t* out = p.page_table + static_cast<int64_t>(row) * p.take;
-  if (tid == 0) {
-    const int64_t left_out = count > p.take ? static_cast<int64_t>(count - p.take) * p.page_size : 0;
-    p.page_lens[row] = static_cast<int32_t>(tokens - left_out);
-  }
+  if (tid == 0) p.page_lens[row] = tokens - (count > p.take ? (count - p.take) * p.page_size : 0);
   if (count <= p.take) {
-    for (int n = tid; n < p.take; n += blockDim.x) out[n] = n < count ? static_cast<int32_t>(page_id(p, b, h, n)) : -1;
+    for (int n = tid; n < p.take; n += kPickThreads) out[n] = n < count ? static_cast<int32_t>(page_id(p, b, 0, n)) : -1;
     return;
   }
   const uint32_t* mine = keys + static_cast<int64_t>(row) * p.table_width;
-  const int others = count - 1;
-  if (tid == 0) s_key = 0, s_left = p.take - 1;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    __syncthreads();
-    if (tid < 256) s_count[tid] = 0;
-    __syncthreads();
-    const uint32_t prefix = s_key;
-    const int left = s_left;
-    for (int n = tid; n < others; n += blockDim.x) {
-      const uint32_t key = mine[n];
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_count[(key >> shift) & 255u], 1);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      int above = 0, digit = 255;
-      for (; digit > 0 && above + s_count[digit] < left; --digit) above += s_count[digit];
-      s_key = prefix | static_cast<uint32_t>(digit) << shift;
-      s_left = left - above;
-    }
+  const int others = count - 1, want = p.take - 1;
+  const int run = kHeld > 0 ? kHeld : (others + kPickThreads - 1) / kPickThreads;
+  const int first = min(tid * run, others), end = min(first + run, others);
+  uint32_t held[kHeld > 0 ? kHeld : 1];
+  if constexpr (kHeld > 0) {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) held[k] = first + k < end ? mine[first + k] : 0u;
   }
+  // `visit` sees this thread's keys; places behind the last count as key 0, below every candidate
+  auto visit = [&](auto&& f) {
+    if constexpr (kHeld > 0) {
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) f(first + k, held[k]);
+    } else {
+      for (int n = first; n < end; ++n) f(n, mine[n]);
+    }
+  };
+  uint32_t least = 0;  // the largest value that at least `want` keys reach
+  int phase = 0;
+  for (int shift = 30; shift >= 0; shift -= 2, phase ^= 1) {
+    const uint32_t one = least | (1u << shift), two = least | (2u << shift), three = least | (3u << shift);
+    int a = 0, c = 0, e = 0;
+    visit([&](int, uint32_t key) { a += key >= one, c += key >= two, e += key >= three; });
+    const int3 reached = cta_sums(a, c, e, s_sum, phase);
+    least = reached.z >= want ? three : reached.y >= want ? two : reached.x >= want ? one : least;
+  }
+  int above = 0, equal = 0;
+  visit([&](int n, uint32_t key) { above += n < end && key > least, equal += n < end && key == least; });
+  // exclusive sums of both over the threads before this one
+  int2 sum = make_int2(above, equal);
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, sum.x, off), y = __shfl_up_sync(0xffffffffu, sum.y, off);
+    if (lane >= off) sum.x += x, sum.y += y;
+  }
+  if (lane == 31) s_scan[warp] = sum;
   __syncthreads();
-  const uint32_t least = s_key;  // the smallest key taken; s_left pages that have it are
-  const int ties = s_left;
-  int written = 0, equal = 0;
-  for (int first = 0; first < others; first += blockDim.x) {
-    const int n = first + tid;
-    const uint32_t key = n < others ? mine[n] : 0u;
-    const bool is_equal = n < others && key == least;
-    const unsigned equal_mask = __ballot_sync(0xffffffffu, is_equal);
-    __syncthreads();
-    if (lane == 0) s_warp[0][warp] = __popc(equal_mask);
-    __syncthreads();
-    int rank = equal;
-    for (int w = 0; w < 32; ++w) rank += w < warp ? s_warp[0][w] : 0, equal += s_warp[0][w];
-    rank += __popc(equal_mask & ((1u << lane) - 1));
-    const bool taken = n < others && (key > least || (is_equal && rank < ties));
-    const unsigned mask = __ballot_sync(0xffffffffu, taken);
-    if (lane == 0) s_warp[1][warp] = __popc(mask);
-    __syncthreads();
-    int at = written;
-    for (int w = 0; w < 32; ++w) at += w < warp ? s_warp[1][w] : 0, written += s_warp[1][w];
-    at += __popc(mask & ((1u << lane) - 1));
-    if (taken) out[at] = static_cast<int32_t>(page_id(p, b, h, n));
+  int before_above = sum.x - above, before_equal = sum.y - equal, all_above = 0;
+#pragma unroll
+  for (int w = 0; w < kPickThreads / 32; ++w) {
+    const int2 x = s_scan[w];
+    if (w < warp) before_above += x.x, before_equal += x.y;
+    all_above += x.x;
   }
-  if (tid == 0) out[p.take - 1] = static_cast<int32_t>(page_id(p, b, h, count - 1));
+  const int ties = want - all_above;  // the first so many of the keys equal to `least`
+  visit([&](int n, uint32_t key) {
+    if (n >= end) return;
+    if (key > least) {
+      out[before_above + min(before_equal, ties)] = static_cast<int32_t>(page_id(p, b, 0, n));
+      ++before_above;
+    } else if (key == least) {
+      if (before_equal < ties) out[before_above + before_equal] = static_cast<int32_t>(page_id(p, b, 0, n));
+      ++before_equal;
+    }
+  });
+  if (tid == 0) out[p.take - 1] = static_cast<int32_t>(page_id(p, b, 0, count - 1));
 }
 
 // Bytes of the keys, a multiple of 16.
@@ -279,8 +354,9 @@ int launch_select(const PagedInt4& p, int head_dim, int dtype, cudaStream_t stre
   const int rows = p.batch * p.kv_heads;
   QF_REQUIRE(rows <= 65535, "at most 65535 (sequence, KV head) rows choose pages in one call");
   uint32_t* keys = static_cast<uint32_t*>(p.workspace);
-  const int64_t blocks = (p.table_width + 63) / 64;
-  const dim3 grid(static_cast<unsigned>(blocks < 1 ? 1 : blocks > 256 ? 256 : blocks), rows);
+  const int64_t pages = head_dim == 128 ? 32 : 64;  // of a CTA at a time
+  const int64_t blocks = (p.table_width + pages - 1) / pages;
+  const dim3 grid(static_cast<unsigned>(blocks < 1 ? 1 : blocks > 2048 ? 2048 : blocks), rows);
   cudaError_t err = cudaSuccess;
   if (dtype == QF_DTYPE_F16) {
     err = head_dim == 128 ? launch_chained(page_score_kernel<__half, 128>, grid, dim3(256), 0, stream, p, keys)
@@ -290,7 +366,15 @@ int launch_select(const PagedInt4& p, int head_dim, int dtype, cudaStream_t stre
                           : launch_chained(page_score_kernel<__nv_bfloat16, 64>, grid, dim3(256), 0, stream, p, keys);
   }
   QF_CUDA(err);
-  QF_CUDA(launch_chained(page_pick_kernel, dim3(rows), dim3(1024), 0, stream, p, static_cast<const uint32_t*>(keys)));
+  const uint32_t* scored = keys;
+  if (p.table_width <= 2 * kPickThreads) {
+    err = launch_chained(page_pick_kernel<2>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored);
+  } else if (p.table_width <= 16 * kPickThreads) {
+    err = launch_chained(page_pick_kernel<16>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored);
+  } else {
+    err = launch_chained(page_pick_kernel<0>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored);
+  }
+  QF_CUDA(err);
   QF_CUDA(cudaGetLastError());
   return QF_OK;
 }
@@ -310,16 +394,17 @@ int qf_int4_key_bounds(const qf_paged_int4_args* args, void* stream) {
   const int64_t spanned = (static_cast<int64_t>(p.new_tokens) + p.page_size - 2) / p.page_size + 1;
   const int pages_each = static_cast<int>(spanned < p.table_width ? spanned : p.table_width);
   const int64_t units = static_cast<int64_t>(p.batch) * p.kv_heads * pages_each;
-  QF_REQUIRE((units + 3) / 4 < (1LL << 31), "too many pages in one call");
+  QF_REQUIRE(units < (1LL << 31) - 4, "too many pages in one call");
   const dim3 grid(static_cast<unsigned>((units + 3) / 4));
+  const Divisor by_each = make_divisor(pages_each);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t err = cudaSuccess;
   if (args->dtype == QF_DTYPE_F16) {
-    err = args->head_dim == 128 ? launch_chained(key_bounds_kernel<__half, 128>, grid, dim3(128), 0, s, p, pages_each)
-                                : launch_chained(key_bounds_kernel<__half, 64>, grid, dim3(128), 0, s, p, pages_each);
+    err = args->head_dim == 128 ? launch_chained(key_bounds_kernel<__half, 128>, grid, dim3(128), 0, s, p, by_each)
+                                : launch_chained(key_bounds_kernel<__half, 64>, grid, dim3(128), 0, s, p, by_each);
   } else {
-    err = args->head_dim == 128 ? launch_chained(key_bounds_kernel<__nv_bfloat16, 128>, grid, dim3(128), 0, s, p, pages_each)
-                                : launch_chained(key_bounds_kernel<__nv_bfloat16, 64>, grid, dim3(128), 0, s, p, pages_each);
+    err = args->head_dim == 128 ? launch_chained(key_bounds_kernel<__nv_bfloat16, 128>, grid, dim3(128), 0, s, p, by_each)
+                                : launch_chained(key_bounds_kernel<__nv_bfloat16, 64>, grid, dim3(128), 0, s, p, by_each);
   }
   QF_CUDA(err);
   QF_CUDA(cudaGetLastError());
@@ -339,7 +424,9 @@ int qf_int4_sparse_decode_attention(const qf_paged_int4_args* args, void* stream
   using namespace qf;
   PagedInt4 p;
   if (const int rc = fill_paged_int4(args, kNeedsQuery | kNeedsPool | kNeedsOut | kNeedsBounds | kNeedsSelection, &p)) return rc;
-  QF_REQUIRE(static_cast<int64_t>(p.take) * p.page_size < (1LL << 31), "the pages taken hold 2^31 tokens or more");
+  QF_REQUIRE(p.take < (1LL << 30) / p.page_size, "the pages taken hold 2^30 tokens or more");
+  QF_REQUIRE(static_cast<int64_t>(p.batch) * p.kv_heads * p.take < (1LL << 30) / (p.page_size / kInt4Tile),
+             "the pages taken hold 2^30 tiles of 16 tokens or more");
   if (p.batch == 0) return QF_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   PagedInt4 next = over_selection(p);

@@ -88,7 +88,7 @@ def _paged_args(cabi, **changes):
     (dict(batch=-1), b"batch"), (dict(q=None), b"aligned"), (dict(q=8), b"aligned"), (dict(q_stride_b=4), b"multiple of 8"),
     (dict(out=None), b"out must"), (dict(pool=8), b"pool must"), (dict(seq_lens=None), b"must not be null"),
     (dict(block_table=None), b"must not be null"), (dict(table_dtype=2), b"page table"), (dict(lens_dtype=2), b"lengths"),
-    (dict(table_width=1 << 28), b"2\\^31 tokens".replace(b"\\", b"")), (dict(num_pages=1 << 31), b"pool or table size"),
+    (dict(table_width=1 << 28), b"2^30 tokens"), (dict(table_width=(1 << 26) - 1, batch=16), b"2^30 tiles"), (dict(take=1 << 26), b"2^30 tokens"), (dict(num_pages=1 << 31), b"pool or table size"),
     (dict(take=0), b"at least one page"), (dict(page_table=None), b"page_table"), (dict(key_bounds=None), b"key bounds"),
     (dict(workspace=None), b"workspace"), (dict(workspace_bytes=8), b"workspace"),
 ])
