@@ -508,7 +508,7 @@ int qf_build_rope_table(float* table, int32_t positions, double base, void* stre
 /* RoPE + quantising cache write: qf_rope_kv_write for this cache (same strides, the same
  * zero queries for rows >= *valid_tokens).  q_heads 0: only K and V.  positions NULL: K is
  * stored as it is (and Q, if any, copied).  rope_table [table_positions][D / 2] (cos, sin)
- * fp32 pairs, or NULL: cosf / sinf of position * base^(-2i / D) as in qf_rope_kv_write; a
+ * fp32 pairs, 16-byte aligned, or NULL: cosf / sinf of position * base^(-2i / D) as in qf_rope_kv_write; a
  * position outside the table is clamped and recorded (status 4).  A rotated key is rounded
  * to T and then quantised.  slot_mapping NULL: slot = row.  A slot outside the pool is
  * skipped.  Two rows of one call with the same slot leave a mixture of both in it. */

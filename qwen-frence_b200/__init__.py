@@ -102,7 +102,9 @@ def kernel_module(name):
 
 def __getattr__(name):
     if name in _EXPORTS:
-        return getattr(kernel_module(_EXPORTS[name]), name)
+        # kept, so that a call does not look its module up again
+        value = globals()[name] = getattr(kernel_module(_EXPORTS[name]), name)
+        return value
     if name == "cabi":
         # one shared instance with the drop-in modules, which load it by path
         return _load("qf_hotpath_cabi", PACKAGE_DIR / "_cabi.py")

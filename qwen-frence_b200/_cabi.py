@@ -263,6 +263,16 @@ def stream_pointer(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def raw_stream(index):
+    """The current torch stream of CUDA device number `index`: stream_pointer without a Stream object."""
+    import torch
+
+    global raw_stream
+    # the call torch's own generated code makes; absent, the public one does
+    raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or stream_pointer
+    return raw_stream(index)
+
+
 class device_of:
     """Make `tensor.device` current for the duration of a library call."""
 

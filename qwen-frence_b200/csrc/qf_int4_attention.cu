@@ -70,6 +70,13 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
+// Largest value of the warp, NaNs left out.
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ float pow2i(int e) {  // 2^e, e in [-126, 127]
   return __int_as_float((e + 127) << 23);
 }
@@ -82,28 +89,6 @@ __device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_g
 template <int N>
 __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ uint64_t pair32(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpair32(uint64_t x) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-  return r;
-}
-// Two products, or products and sums, in one instruction.
-__device__ __forceinline__ uint64_t mul32x2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma32x2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
 }
 
 // What a call shares out: units of all rows (fewer than 2^31), units of a CTA.
@@ -363,8 +348,7 @@ struct Row {
 
   // Raise the offset to this unit's largest scores and steps.
   __device__ __forceinline__ void raise(const float (&x)[NT][8], float magnitude, int left, int g) {
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) magnitude = fmaxf(magnitude, __shfl_xor_sync(0xffffffffu, magnitude, d));
+    magnitude = warp_max(magnitude);
     const int above = max(-60, (__float_as_int(magnitude) >> 23) - 126);  // magnitude < 2^above
     const int next = max(e, min(above, 100));
 #pragma unroll
@@ -607,6 +591,13 @@ struct Merge {
       x[0] = v.x, x[1] = v.y;
     }
   }
+  static __device__ __forceinline__ void store(float* at, const float (&x)[C]) {
+    if constexpr (C == 4) {
+      *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+      *reinterpret_cast<float2*>(at) = make_float2(x[0], x[1]);
+    }
+  }
   template <typename T>
   __device__ __forceinline__ void write_out(const PagedInt4& p, int row, int group, int head, int lane, float sum) const {
     const int2 at = row_place(p, row);
@@ -623,11 +614,6 @@ struct Merge {
   }
 };
 
-__device__ __forceinline__ float warp_max(float x) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-  return x;
-}
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
@@ -667,7 +653,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
   uint8_t* ring = s_ring + warp * S::kRing;
   if (threadIdx.x < 2 * kWarps) s_row[threadIdx.x] = -1;
   release_dependents();
-  dependency_wait();
+  if (!p.early) dependency_wait();
   const Plan plan = make_plan(p, s_shares, chunk, ctas);
 
   // this warp's units
@@ -676,8 +662,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
   const int first = cta_first + static_cast<int>(static_cast<int64_t>(cta_units) * warp / kWarps);
   const int units = cta_first + static_cast<int>(static_cast<int64_t>(cta_units) * (warp + 1) / kWarps) - first;
 
+  Requests ahead{};
   if (units > 0) {
-    Requests ahead;
     {
       const int2 found = find_rows(s_shares, first, lane);
       ahead.row = found.x * chunk;
@@ -694,12 +680,16 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
       ahead.unit = before;
       ahead.left = units;
     }
-    Lengths lengths = ahead.lengths;
-    int id = ahead.row, in_row = ahead.unit;  // of the unit at hand
+  }
+  Lengths lengths = ahead.lengths;
+  int id = ahead.row, in_row = ahead.unit;  // of the unit at hand
+  if (units > 0) ahead.refill(p, lane);
+  if (p.early) dependency_wait();
+
+  if (units > 0) {
     Row<T, D, NT> row;
     uint4 queries[NT][D / kInt4Group];
     row.load(p, id, group, lane, queries);
-    ahead.refill(p, lane);
 
     int wanted = 0;                                     // units requested
     uint32_t request_at = smem_u32(ring) + 16 * lane;  // where this lane's part of the next goes
@@ -771,14 +761,15 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
   }
   __syncthreads();
 
-  // Rows that several warps, or several CTAs, hold: a warp takes the head with its number, a lane
-  // the offset and the sum of one piece.
+  // Rows that several warps, or several CTAs, hold: a warp takes a head, a lane the offset and the
+  // sum of one piece.
   const int my_row = lane < 2 * kWarps ? s_row[lane] : -1;
   const int my_flags = my_row >= 0 ? s_flags[lane] : 0;
   const float* warp_pieces = scratch.warp_pieces + static_cast<int64_t>(cta) * kWarps * S::kPiece;
   auto piece_of = [&](int k) {
     return (k & 1) ? reinterpret_cast<const float*>(s_ring + (k >> 1) * S::kRing) : warp_pieces + (k >> 1) * S::kPiece;
   };
+  int item = 0;  // (chain, head) pairs are dealt out to the warps in turn
   for (unsigned rest = __ballot_sync(0xffffffffu, my_row >= 0); rest != 0u;) {
     const int i = __ffs(rest) - 1;
     const int id = __shfl_sync(0xffffffffu, my_row, i);
@@ -786,21 +777,19 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
     rest &= ~chain;
     const bool starts = (__shfl_sync(0xffffffffu, my_flags, i) & kRowStart) != 0;
     const bool ends = (__shfl_sync(0xffffffffu, my_flags, 31 - __clz(chain)) & kRowEnd) != 0;
-#pragma unroll
-    for (int nt = 0; nt < (S::kHeads + kWarps - 1) / kWarps; ++nt) {
-      const int head = kWarps * nt + warp;  // eight warps and more: a head a warp, twice for 16 heads
-      if (head >= group) break;
+    int head = (warp - item) & (kWarps - 1);
+    item += group;
+    for (; head < group; head += kWarps) {
       float2 ml = make_float2(-INFINITY, 0.f);
       if (my_row == id) ml = *reinterpret_cast<const float2*>(piece_of(lane) + S::kHeads * S::kStride + 2 * head);
-      const float top = warp_max(ml.x);
-      const float weight = my_row == id ? fast_exp2(ml.x - top) : 0.f;
-      const float sum = warp_sum(ml.y * weight);
       Merge<D> merge;
       merge.clear();
+      const float top = warp_max(ml.x);
+      const float weight = my_row == id ? fast_exp2(ml.x - top) : 0.f;
       for (unsigned left = chain; left != 0u;) {
         float x[4][Merge<D>::C], scale[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {  // four pieces in flight; the last one again, weightless, where fewer are left
+        for (int n = 0; n < 4; ++n) {  // four pieces in flight; the first one again, weightless, where fewer are left
           const int k = left != 0u ? __ffs(left) - 1 : i;
           scale[n] = __shfl_sync(0xffffffffu, weight, k);
           if (left == 0u) scale[n] = 0.f;
@@ -810,12 +799,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
 #pragma unroll
         for (int n = 0; n < 4; ++n) merge.add(x[n], scale[n]);
       }
+      const float sum = warp_sum(ml.y * weight);
       if (starts && ends) {
         merge.template write_out<T>(p, id, group, head, lane, sum);
       } else {
         float* piece = scratch.cta_pieces + static_cast<int64_t>(2 * cta + (starts ? 1 : 0)) * S::kPiece;
-#pragma unroll
-        for (int c = 0; c < Merge<D>::C; ++c) piece[head * S::kStride + lane * Merge<D>::C + c] = merge.o[c];
+        Merge<D>::store(piece + head * S::kStride + lane * Merge<D>::C, merge.o);
         if (lane == 0) *reinterpret_cast<float2*>(piece + S::kHeads * S::kStride + 2 * head) = make_float2(top, sum);
       }
     }
@@ -831,13 +820,15 @@ __global__ void __launch_bounds__(128) int4_combine_kernel(const PagedInt4 p, in
   __shared__ float s_o[4][D];
   __shared__ float s_top[4], s_sum[4];
   release_dependents();
-  dependency_wait();
+  if (!p.early) dependency_wait();
   const int group = by_group.d;
   const int row = quotient(blockIdx.x, by_group), head = blockIdx.x - row * group;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Scratch scratch = carve<D, NT>(p.workspace, ctas);
+  const int tokens = row_tokens_at(p, row);
+  if (p.early) dependency_wait();
   const int2 span = scratch.spans[row];  // unwritten, and not used, for a row without tokens
-  if (row_tokens_at(p, row) == 0) {
+  if (tokens == 0) {
     const int2 at = row_place(p, row);
     T* dst = static_cast<T*>(p.out) + at.x * p.o_sb + (static_cast<int64_t>(at.y) * group + head) * p.o_sh;
     for (int d = threadIdx.x; d < D; d += 128) dst[d] = from_float<T>(0.f);

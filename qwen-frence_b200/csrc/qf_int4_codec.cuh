@@ -33,64 +33,106 @@ constexpr float kInt4MinStep = 8.673617379884035e-19f;  // 2^-60
 __host__ __device__ constexpr int int4_tile_bytes(int head_dim) { return 20 * head_dim; }
 
 struct Int4Group {
-  float step, low;  // values of type T
-  bool finite;
+  float step, low;  // values of type T, NaN where the group is not finite
 };
 
-// step and floor of a group from its extremes (values of T), rounded to T as they are held.
+// Minimum and maximum that keep a NaN, of three.
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Correctly rounded x / d from y, the correctly rounded 1 / d: q = x y, and the exact remainder
+// x - q d times y added to it (Markstein, "Computation of elementary functions on the IBM RISC
+// System/6000", 1990; a d of 11 bits or fewer is never the all-ones mantissa it excludes).
+__device__ __forceinline__ float divide_by(float x, float d, float y) {
+  const float q = __fmul_rn(x, y);
+  return __fmaf_rn(__fmaf_rn(-q, d, x), y, q);
+}
+
+// step and floor of a group from its extremes (values of T, NaN if the group holds one), rounded
+// to T as they are held.
 template <typename T>
-__device__ __forceinline__ Int4Group int4_group(float low, float high, bool finite) {
+__device__ __forceinline__ Int4Group int4_group(float low, float high) {
   Int4Group g;
-  const float step = to_float(from_float<T>(__fdiv_rn(__fsub_rn(high, low), 15.f)));
+  const float range = __fsub_rn(high, low);
+  const float step = to_float(from_float<T>(divide_by(range, 15.f, 1.f / 15.f)));
+  const bool finite = range <= 3.402823466e38f;
   g.step = finite ? (step < kInt4MinStep ? 0.f : step) : __int_as_float(0x7fc00000);
   g.low = finite ? low : __int_as_float(0x7fc00000);
-  g.finite = finite;
   return g;
 }
 
-// rint(x / step) as the nearest integers of correctly rounded quotients: T's coarse grid puts
-// many quotients exactly between two codes, and the product with a rounded reciprocal alone
-// would tip those either way.  With y the correctly rounded 1 / step, q = x y and the exact
-// remainder x - q step, q + remainder * y is the correctly rounded quotient (Markstein, "Computation
-// of elementary functions on the IBM RISC System/6000", 1990; steps of 11 bits at most are never
-// the all-ones mantissa it excludes).  Adding 1.5 * 2^23 rounds to an integer, ties to even.
-__device__ __forceinline__ float int4_code(float x, const Int4Group& g, float inverse) {
-  const float t = __fsub_rn(x, g.low);
-  const float q = __fmul_rn(t, inverse);
-  const float n = __fmaf_rn(__fmaf_rn(-q, g.step, t), inverse, q);
-  return __fsub_rn(__fadd_rn(fminf(n, 15.f), 12582912.f), 12582912.f);
-}
-
-// Eight codes as one word, the first in the low bits.  The sums are whole numbers below 2^16.
+// Eight codes as one word, the first in the low bits.  T's coarse grid puts many quotients exactly
+// between two codes, and the product with a rounded reciprocal alone would tip those either way:
+// the quotients are correctly rounded.  Adding 1.5 * 2^23 rounds to an integer, ties to even; four
+// codes are summed as one number below 2^16 and read off the mantissa of 2^23.
 __device__ __forceinline__ uint32_t int4_word(const float (&x)[8], const Int4Group& g) {
-  if (!g.finite || g.step == 0.f) return 0u;
+  if (!(g.step > 0.f)) return 0u;
   const float inverse = __frcp_rn(g.step);
-  float half[2];
+  uint32_t half[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    half[k] = int4_code(x[4 * k + 3], g, inverse);
+    float sum = 0.f;
 #pragma unroll
-    for (int j = 2; j >= 0; --j) half[k] = __fmaf_rn(half[k], 16.f, int4_code(x[4 * k + j], g, inverse));
+    for (int j = 3; j >= 0; --j) {
+      const float n = fminf(divide_by(__fsub_rn(x[4 * k + j], g.low), g.step, inverse), 15.f);
+      sum = __fmaf_rn(sum, 16.f, __fsub_rn(__fadd_rn(n, 12582912.f), 12582912.f));
+    }
+    half[k] = __float_as_uint(__fadd_rn(sum, 8388608.f));
   }
-  return static_cast<uint32_t>(half[0]) | static_cast<uint32_t>(half[1]) << 16;
+  return __byte_perm(half[0], half[1], 0x5410);
 }
 
-// Four codes (bits 0..15 of `word`) as floats n, 16 n, 256 n, 4096 n: the bits laid into the
-// mantissa of 2^23.  Products with step / 1, 16, 256, 4096 are those of n and step.
-__device__ __forceinline__ void int4_scaled(uint32_t word, float (&n)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) n[j] = __fsub_rn(__uint_as_float((word & (15u << (4 * j))) | 0x4b000000u), 8388608.f);
+__device__ __forceinline__ uint64_t pair32(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair32(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+// Two products, sums, or products and sums in one instruction, each rounded once.
+__device__ __forceinline__ uint64_t mul32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
-// The values of eight codes.  n * step is exact in fp32 (4 + 11 bits), so each is one rounding.
+// The values of eight codes.  Four codes laid into the mantissa of 2^23 are n, 16 n, 256 n and
+// 4096 n above it; with step / 1, 16, 256 and 4096 their products are those of n and step, exact in
+// fp32 (4 + 11 bits), so each value is one rounding.
 __device__ __forceinline__ void int4_values(uint32_t word, float step, float low, float (&x)[8]) {
-  const float steps[4] = {step, step * 0.0625f, step * 0.00390625f, step * 0.000244140625f};
+  const uint64_t steps[2] = {pair32(step, step * 0.0625f), pair32(step * 0.00390625f, step * 0.000244140625f)};
+  const uint64_t lows = pair32(low, low), minus = pair32(-8388608.f, -8388608.f);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    float n[4];
-    int4_scaled(word >> (16 * k), n);
+    const uint32_t half = word >> (16 * k);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[4 * k + j] = __fmaf_rn(n[j], steps[j], low);
+    for (int j = 0; j < 2; ++j) {
+      const uint64_t n = add32x2(pair32(__uint_as_float((half & (15u << (8 * j))) | 0x4b000000u),
+                                        __uint_as_float((half & (240u << (8 * j))) | 0x4b000000u)), minus);
+      const float2 two = unpair32(fma32x2(n, steps[j], lows));
+      x[4 * k + 2 * j] = two.x, x[4 * k + 2 * j + 1] = two.y;
+    }
   }
 }
 

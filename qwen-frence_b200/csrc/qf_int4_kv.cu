@@ -35,95 +35,112 @@ struct WriteParams {
 
 constexpr int kWriteThreads = 256;
 
-__device__ __forceinline__ bool finite32(float x) { return fabsf(x) <= 3.402823466e38f; }
+// Where the angles of a call come from.
+enum : int { kNoRope, kTable, kAngles };
 
 // Rows and their segments (heads) are laid end to end: a segment takes D / 16 threads, each with
 // the eight channels at d0 and the eight they rotate with at d0 + D / 2, so a CTA of 256 covers
 // two rows of 12 + 2 + 2 heads and no thread idles.  A group of 32 channels is four neighbouring
-// threads, whose extremes meet in two shuffles.  The CTA's cosines and sines go through shared
-// memory: 14 heads of a row use each.
-template <typename T, int D, bool VEC>
+// threads, whose extremes meet in two shuffles.  A thread fetches its cosines and sines from the
+// table itself (a row's 14 rotated heads hit the first level cache; passing them through shared
+// memory instead costs a barrier behind two dependent loads); without a table the CTA computes
+// each once and shares it.
+template <typename T, int D, bool VEC, int ROPE>
 __global__ void __launch_bounds__(kWriteThreads) int4_write_kernel(const WriteParams p, const __grid_constant__ InvFreqTable freq) {
   constexpr int kHalf = D / 2, kLanes = D / 16, W = D / kInt4Group;
-  constexpr int kRows = kWriteThreads / (2 * kLanes) + 1;  // one KV head and no query heads: the most rows a CTA meets
-  __shared__ float2 s_rope[kRows][kHalf];
   release_dependents();
   dependency_wait();
   const uint32_t first = blockIdx.x * kWriteThreads;
-  const int first_row = quotient(first, p.items);
   const int index = first + threadIdx.x;
   const int row = quotient(index, p.items);
   const bool on = row < p.rows;
   const int item = index - row * p.items.d;
   const int live_rows = p.valid_tokens ? min(*p.valid_tokens, p.rows) : p.rows;
   const bool live = row < live_rows;
-  int64_t slot = -1;
-  if (live) slot = p.slots != nullptr ? load_index(p.slots, p.slot_dtype, row * p.slot_stride) : row;
-  const bool slot_ok = slot >= 0 && slot < p.num_slots;
   const int segment = item / kLanes, d0 = (item % kLanes) * 8;
   const bool is_q = segment < p.q_heads;
   const bool is_k = !is_q && segment < p.q_heads + p.kv_heads;
   const int head = is_q ? segment : is_k ? segment - p.q_heads : segment - p.q_heads - p.kv_heads;
-  const T* src;
-  int64_t sd;
-  if (is_q) {
-    src = static_cast<const T*>(p.q) + row * p.q_sr + head * p.q_sh, sd = p.q_sd;
-  } else if (is_k) {
-    src = static_cast<const T*>(p.k) + row * p.k_sr + head * p.k_sh, sd = p.k_sd;
-  } else {
-    src = static_cast<const T*>(p.v) + row * p.v_sr + head * p.v_sh, sd = p.v_sd;
-  }
-  alignas(16) T x[16];
-  if (live && (is_q || slot_ok)) {
-    if constexpr (VEC) {
-      *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(src + d0);
-      *reinterpret_cast<uint4*>(x + 8) = *reinterpret_cast<const uint4*>(src + d0 + kHalf);
+  int64_t position = 0;
+  if (ROPE == kTable && live) position = load_index(p.positions, p.pos_dtype, row * p.pos_stride);
+  int64_t slot = -1;
+  if (live && !is_q) slot = p.slots != nullptr ? load_index(p.slots, p.slot_dtype, row * p.slot_stride) : row;
+  const bool slot_ok = slot >= 0 && slot < p.num_slots;
+  // eight channels and the eight they rotate with, two to a register
+  uint32_t x[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  if (live) {
+    const T* src;
+    int64_t sd;
+    if (is_q) {
+      src = static_cast<const T*>(p.q) + row * p.q_sr + head * p.q_sh, sd = p.q_sd;
+    } else if (is_k) {
+      src = static_cast<const T*>(p.k) + row * p.k_sr + head * p.k_sh, sd = p.k_sd;
     } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = src[(d0 + j) * sd], x[8 + j] = src[(d0 + kHalf + j) * sd];
+      src = static_cast<const T*>(p.v) + row * p.v_sr + head * p.v_sh, sd = p.v_sd;
     }
-  } else {
+    if constexpr (VEC) {
+      *reinterpret_cast<uint4*>(x[0]) = *reinterpret_cast<const uint4*>(src + d0);
+      *reinterpret_cast<uint4*>(x[1]) = *reinterpret_cast<const uint4*>(src + d0 + kHalf);
+    } else {
+      const uint16_t* bits = reinterpret_cast<const uint16_t*>(src);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = from_float<T>(0.f);
+      for (int j = 0; j < 8; ++j) {
+        x[j / 4][j % 4] = bits[(d0 + j / 4 * kHalf + 2 * (j % 4)) * sd] |
+                          static_cast<uint32_t>(bits[(d0 + j / 4 * kHalf + 2 * (j % 4) + 1) * sd]) << 16;
+      }
+    }
   }
 
-  if (p.positions != nullptr) {
-    const int last_row = min(static_cast<int>(quotient(first + kWriteThreads - 1, p.items)), live_rows - 1);
-    for (int i = threadIdx.x; i < (last_row - first_row + 1) * kHalf; i += kWriteThreads) {
-      const int r = i / kHalf, f = i % kHalf;
-      if (p.table != nullptr) {
-        int64_t position = load_index(p.positions, p.pos_dtype, (first_row + r) * p.pos_stride);
+  if constexpr (ROPE != kNoRope) {
+    const bool turns = live && (is_q || is_k);
+    float4 cs[4];  // (cos, sin) of channels d0 + 2 j and d0 + 2 j + 1
+    if constexpr (ROPE == kTable) {
+      if (turns) {
         if (position < 0 || position >= p.table_positions) {
           position = position < 0 ? 0 : p.table_positions - 1;
-          if (f == 0) atomicMax(p.status, kStatusPositionPastTable);
+          atomicMax(p.status, kStatusPositionPastTable);
         }
-        s_rope[r][f] = p.table[position * kHalf + f];
-      } else {
+        const float4* at = reinterpret_cast<const float4*>(p.table + position * kHalf + d0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) cs[j] = at[j];
+      }
+    } else {
+      constexpr int kRows = kWriteThreads / (2 * kLanes) + 1;  // one KV head and no query heads: the most rows a CTA meets
+      __shared__ __align__(16) float2 s_rope[kRows][kHalf];
+      const int first_row = quotient(first, p.items);
+      const int last_row = min(static_cast<int>(quotient(first + kWriteThreads - 1, p.items)), live_rows - 1);
+      for (int i = threadIdx.x; i < (last_row - first_row + 1) * kHalf; i += kWriteThreads) {
+        const int r = i / kHalf, f = i % kHalf;
         const float angle = __fmul_rn(load_position(p.positions, p.pos_dtype, (first_row + r) * p.pos_stride), freq.v[f]);
         s_rope[r][f] = make_float2(cosf(angle), sinf(angle));
       }
-    }
-    __syncthreads();
-    if (live && (is_q || is_k)) {
+      __syncthreads();
+      if (turns) {
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const float4 cs = *reinterpret_cast<const float4*>(&s_rope[row - first_row][d0 + j]);
-        const float a0 = to_float(x[j]), b0 = to_float(x[8 + j]), a1 = to_float(x[j + 1]), b1 = to_float(x[9 + j]);
-        x[j] = from_float<T>(__fsub_rn(__fmul_rn(a0, cs.x), __fmul_rn(b0, cs.y)));
-        x[8 + j] = from_float<T>(__fadd_rn(__fmul_rn(b0, cs.x), __fmul_rn(a0, cs.y)));
-        x[j + 1] = from_float<T>(__fsub_rn(__fmul_rn(a1, cs.z), __fmul_rn(b1, cs.w)));
-        x[9 + j] = from_float<T>(__fadd_rn(__fmul_rn(b1, cs.z), __fmul_rn(a1, cs.w)));
+        for (int j = 0; j < 4; ++j) cs[j] = *reinterpret_cast<const float4*>(&s_rope[row - first_row][d0 + 2 * j]);
+      }
+    }
+    if (turns) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = unpack2<T>(x[0][j]), b = unpack2<T>(x[1][j]);
+        x[0][j] = pack2<T>(__fsub_rn(__fmul_rn(a.x, cs[j].x), __fmul_rn(b.x, cs[j].y)), __fsub_rn(__fmul_rn(a.y, cs[j].z), __fmul_rn(b.y, cs[j].w)));
+        x[1][j] = pack2<T>(__fadd_rn(__fmul_rn(b.x, cs[j].x), __fmul_rn(a.x, cs[j].y)), __fadd_rn(__fmul_rn(b.y, cs[j].z), __fmul_rn(a.y, cs[j].w)));
       }
     }
   }
   if (on && is_q) {
     T* dst = static_cast<T*>(p.q_out) + row * p.o_sr + head * p.o_sh;
     if constexpr (VEC) {
-      *reinterpret_cast<uint4*>(dst + d0) = *reinterpret_cast<uint4*>(x);
-      *reinterpret_cast<uint4*>(dst + d0 + kHalf) = *reinterpret_cast<uint4*>(x + 8);
+      *reinterpret_cast<uint4*>(dst + d0) = *reinterpret_cast<uint4*>(x[0]);
+      *reinterpret_cast<uint4*>(dst + d0 + kHalf) = *reinterpret_cast<uint4*>(x[1]);
     } else {
+      uint16_t* bits = reinterpret_cast<uint16_t*>(dst);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dst[(d0 + j) * p.o_sd] = x[j], dst[(d0 + kHalf + j) * p.o_sd] = x[8 + j];
+      for (int j = 0; j < 8; ++j) {
+        bits[(d0 + j / 4 * kHalf + 2 * (j % 4)) * p.o_sd] = static_cast<uint16_t>(x[j / 4][j % 4]);
+        bits[(d0 + j / 4 * kHalf + 2 * (j % 4) + 1) * p.o_sd] = static_cast<uint16_t>(x[j / 4][j % 4] >> 16);
+      }
     }
   }
   if (__all_sync(0xffffffffu, is_q || !slot_ok)) return;
@@ -136,23 +153,20 @@ __global__ void __launch_bounds__(kWriteThreads) int4_write_kernel(const WritePa
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     float f[8];
-    float low, high;
-    bool finite = true;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      f[j] = to_float(x[8 * side + j]);
-      low = j == 0 ? f[j] : fminf(low, f[j]);
-      high = j == 0 ? f[j] : fmaxf(high, f[j]);
-      finite = finite && finite32(f[j]);
+    for (int j = 0; j < 4; ++j) {
+      const float2 two = unpack2<T>(x[side][j]);
+      f[2 * j] = two.x, f[2 * j + 1] = two.y;
     }
+    float low = min_nan(min_nan(f[0], f[1], f[2]), min_nan(f[3], f[4], f[5]), min_nan(f[6], f[7], f[7]));
+    float high = max_nan(max_nan(f[0], f[1], f[2]), max_nan(f[3], f[4], f[5]), max_nan(f[6], f[7], f[7]));
 #pragma unroll
     for (int off = 1; off <= 2; off <<= 1) {
-      low = fminf(low, __shfl_xor_sync(0xffffffffu, low, off));
-      high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, off));
-      finite = __shfl_xor_sync(0xffffffffu, finite ? 1 : 0, off) != 0 && finite;
+      const float a = __shfl_xor_sync(0xffffffffu, low, off), z = __shfl_xor_sync(0xffffffffu, high, off);
+      low = min_nan(low, a, a), high = max_nan(high, z, z);
     }
     if (is_q || !slot_ok) continue;
-    const Int4Group g = int4_group<T>(low, high, finite);
+    const Int4Group g = int4_group<T>(low, high);
     const uint32_t word = int4_word(f, g);
     const int channel = d0 + side * kHalf;
     const int w = channel / kInt4Group, t = channel % kInt4Group / 8;
@@ -171,43 +185,85 @@ __global__ void __launch_bounds__(kWriteThreads) int4_write_kernel(const WritePa
   }
 }
 
-// Rows at a list of slots as 16-bit K and V.  A thread takes eight channels of one row of K
-// and of V: 16-byte stores side by side.  A slot outside the pool gives a row of zeros.
+// W 32-bit words, W 16-bit elements.
+template <int W>
+__device__ __forceinline__ void load_words(const uint8_t* at, uint32_t (&x)[W]) {
+  if constexpr (W == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(at);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    x[0] = v.x, x[1] = v.y;
+  }
+}
+template <typename T, int W>
+__device__ __forceinline__ void load_elements(const uint8_t* at, float (&x)[W]) {
+  uint32_t bits[W / 2];
+  if constexpr (W == 4) {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    bits[0] = v.x, bits[1] = v.y;
+  } else {
+    bits[0] = *reinterpret_cast<const uint32_t*>(at);
+  }
+#pragma unroll
+  for (int j = 0; j < W / 2; ++j) {
+    const float2 two = unpack2<T>(bits[j]);
+    x[2 * j] = two.x, x[2 * j + 1] = two.y;
+  }
+}
+
+// Rows at a list of slots as 16-bit K and V.  Four threads a row and head, eight channels of every
+// group each: seven loads bring a thread's D / 2 values, and its stores are 16 bytes beside its
+// neighbours'.  A slot outside the pool gives a row of zeros.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) int4_read_kernel(const uint8_t* __restrict__ pool, const void* __restrict__ slots,
                                                         int slot_dtype, int64_t slot_stride, int rows, int64_t num_slots,
                                                         const Divisor kv_heads, const Divisor page_size,
                                                         T* __restrict__ k_out, T* __restrict__ v_out) {
-  constexpr int kLanes = D / 8, W = D / kInt4Group;
+  constexpr int W = D / kInt4Group;
   release_dependents();
   dependency_wait();
-  const uint32_t segment = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  const int lane = threadIdx.x % kLanes;
+  const uint32_t segment = blockIdx.x * 64 + threadIdx.x / 4;
+  const int t = threadIdx.x % 4;
   const int row = quotient(segment, kv_heads);
   const int head = segment - row * kv_heads.d;
   if (row >= rows) return;
   const int64_t slot = slots != nullptr ? load_index(slots, slot_dtype, row * slot_stride) : row;
-  uint4 k = make_uint4(0, 0, 0, 0), v = k;
-  if (slot >= 0 && slot < num_slots) {
-    const uint32_t page = quotient(static_cast<uint32_t>(slot), page_size);
-    const int in_page = static_cast<int>(static_cast<uint32_t>(slot) - page * page_size.d), token = in_page % kInt4Tile;
-    const uint8_t* tile = pool + ((static_cast<int64_t>(page) * kv_heads.d + head) * (page_size.d / kInt4Tile) + in_page / kInt4Tile) *
-                                     int4_tile_bytes(D);
-    const int w = lane / 4, t = lane % 4;
-    const T* params = reinterpret_cast<const T*>(tile + 16 * D) + token * W + w;
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(tile + token * (D / 2) + t * 4 * W + 4 * w);
-    const uint8_t* vp = tile + 8 * D + token / 2 * D + 2 * t * 4 * W + 4 * w + token % 2 * 2;
-    const uint32_t vw = *reinterpret_cast<const uint16_t*>(vp) |
-                        static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(vp + 4 * W)) << 16;
-    float x[8];
-    int4_values(kw, to_float(params[0]), to_float(params[D / 2]), x);
-    k = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
-    int4_values(vw, to_float(params[D]), to_float(params[3 * D / 2]), x);
-    v = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+  T* k_at = k_out + static_cast<int64_t>(segment) * D + 8 * t;
+  T* v_at = v_out + static_cast<int64_t>(segment) * D + 8 * t;
+  if (slot < 0 || slot >= num_slots) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      *reinterpret_cast<uint4*>(k_at + 32 * w) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(v_at + 32 * w) = make_uint4(0, 0, 0, 0);
+    }
+    return;
   }
-  const int64_t at = static_cast<int64_t>(segment) * D + lane * 8;
-  *reinterpret_cast<uint4*>(k_out + at) = k;
-  *reinterpret_cast<uint4*>(v_out + at) = v;
+  const uint32_t page = quotient(static_cast<uint32_t>(slot), page_size);
+  const int in_page = static_cast<int>(static_cast<uint32_t>(slot) - page * page_size.d), token = in_page % kInt4Tile;
+  const uint8_t* tile = pool + ((static_cast<int64_t>(page) * kv_heads.d + head) * (page_size.d / kInt4Tile) + in_page / kInt4Tile) *
+                                   int4_tile_bytes(D);
+  uint32_t k[W], even[W], odd[W];  // K words, V words of channels 8t..8t + 3 and 8t + 4..8t + 7 of every group
+  load_words<W>(tile + token * (D / 2) + t * 4 * W, k);
+  load_words<W>(tile + 8 * D + token / 2 * D + 2 * t * 4 * W, even);
+  load_words<W>(tile + 8 * D + token / 2 * D + (2 * t + 1) * 4 * W, odd);
+  float steps[2][W], floors[2][W];
+  const uint8_t* params = tile + 16 * D + token * 2 * W;
+  load_elements<T, W>(params, steps[0]);
+  load_elements<T, W>(params + D, floors[0]);
+  load_elements<T, W>(params + 2 * D, steps[1]);
+  load_elements<T, W>(params + 3 * D, floors[1]);
+  const uint32_t which = token % 2 ? 0x7632u : 0x5410u;  // the halves of the pair's words that are this token's
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    float x[8];
+    int4_values(k[w], steps[0][w], floors[0][w], x);
+    *reinterpret_cast<uint4*>(k_at + 32 * w) =
+        make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+    int4_values(__byte_perm(even[w], odd[w], which), steps[1][w], floors[1][w], x);
+    *reinterpret_cast<uint4*>(v_at + 32 * w) =
+        make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+  }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -237,6 +293,7 @@ int launch_write(const qf_int4_write_args* a, cudaStream_t stream) {
                "positions must be int32, int64, or (without a table) float32");
     QF_REQUIRE(a->rope_table != nullptr || a->base > 0.0, "rope base must be positive");
     QF_REQUIRE(a->rope_table == nullptr || a->table_positions >= 1, "the RoPE table is empty");
+    QF_REQUIRE(aligned16(a->rope_table), "the RoPE table must be 16-byte aligned");
   }
   QF_REQUIRE(a->slot_mapping == nullptr || a->slot_dtype == QF_INDEX_I32 || a->slot_dtype == QF_INDEX_I64,
              "slot mapping must use an integer dtype");
@@ -268,15 +325,26 @@ int launch_write(const qf_int4_write_args* a, cudaStream_t stream) {
   }
   const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a->rows) * items + kWriteThreads - 1) / kWriteThreads));
   cudaError_t err = cudaSuccess;
-#define QF_LAUNCH_WRITE(T, D)                                                                             \
-  err = vec ? launch_chained(int4_write_kernel<T, D, true>, grid, dim3(kWriteThreads), 0, stream, p, freq) \
-            : launch_chained(int4_write_kernel<T, D, false>, grid, dim3(kWriteThreads), 0, stream, p, freq)
+#define QF_LAUNCH_WRITE_AS(T, D, ROPE)                                                                              \
+  err = vec ? launch_chained(int4_write_kernel<T, D, true, ROPE>, grid, dim3(kWriteThreads), 0, stream, p, freq)     \
+            : launch_chained(int4_write_kernel<T, D, false, ROPE>, grid, dim3(kWriteThreads), 0, stream, p, freq)
+#define QF_LAUNCH_WRITE(T, D)                     \
+  do {                                            \
+    if (a->positions == nullptr) {                \
+      QF_LAUNCH_WRITE_AS(T, D, kNoRope);          \
+    } else if (a->rope_table != nullptr) {        \
+      QF_LAUNCH_WRITE_AS(T, D, kTable);           \
+    } else {                                      \
+      QF_LAUNCH_WRITE_AS(T, D, kAngles);          \
+    }                                             \
+  } while (0)
   if (a->dtype == QF_DTYPE_F16) {
     if (a->head_dim == 128) QF_LAUNCH_WRITE(__half, 128); else QF_LAUNCH_WRITE(__half, 64);
   } else {
     if (a->head_dim == 128) QF_LAUNCH_WRITE(__nv_bfloat16, 128); else QF_LAUNCH_WRITE(__nv_bfloat16, 64);
   }
 #undef QF_LAUNCH_WRITE
+#undef QF_LAUNCH_WRITE_AS
   QF_CUDA(err);
   QF_CUDA(cudaGetLastError());
   return QF_OK;
@@ -305,8 +373,7 @@ int qf_int4_read_rows(const void* pool, int64_t num_pages, int32_t page_size, in
   QF_REQUIRE(pool && k_out && v_out, "pool, k_out and v_out must not be null");
   QF_REQUIRE(aligned16(pool) && aligned16(k_out) && aligned16(v_out), "pool and outputs must be 16-byte aligned");
   QF_REQUIRE(rows < (1LL << 31) / kv_heads - 256, "too many rows in one call");
-  const int64_t items = rows * kv_heads * (head_dim / 8);
-  const dim3 grid(static_cast<unsigned>((items + 255) / 256));
+  const dim3 grid(static_cast<unsigned>((rows * kv_heads + 63) / 64));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const uint8_t* bytes = static_cast<const uint8_t*>(pool);
   cudaError_t err = cudaSuccess;

@@ -46,6 +46,9 @@ int fill_paged_int4(const qf_paged_int4_args* a, int needs, PagedInt4* p) {
     }
     if (needs & kNeedsSelection) {
       QF_REQUIRE(a->take >= 1, "at least one page must be taken");
+      QF_REQUIRE(a->take < (1LL << 30) / a->page_size, "the pages taken hold 2^30 tokens or more");
+      QF_REQUIRE(static_cast<int64_t>(a->batch) * a->kv_heads * a->take < (1LL << 30) / (a->page_size / kInt4Tile),
+                 "the pages taken hold 2^30 tiles of 16 tokens or more");
       QF_REQUIRE(a->page_table && a->page_lens, "page_table and page_lens must not be null");
     }
   }
@@ -61,6 +64,7 @@ int fill_paged_int4(const qf_paged_int4_args* a, int needs, PagedInt4* p) {
   r.batch = a->batch, r.q_heads = a->q_heads, r.kv_heads = a->kv_heads, r.page_size = a->page_size;
   r.table_dtype = a->table_dtype, r.lens_dtype = a->lens_dtype;
   r.new_tokens = a->new_tokens, r.take = a->take;
+  r.early = true;
   r.by_heads = make_divisor(a->kv_heads), r.by_page = make_divisor(a->page_size);
   r.by_tiles = make_divisor(a->page_size / kInt4Tile);
   if (a->batch > 0) {
@@ -73,63 +77,64 @@ int fill_paged_int4(const qf_paged_int4_args* a, int needs, PagedInt4* p) {
 
 namespace {
 
-// The extremes of a page keep a NaN: a page that holds one must not look harmless.
-__device__ __forceinline__ float max_nan(float a, float b) {
+// Extremes and scores keep a NaN: a page that holds one must not look harmless.
+__device__ __forceinline__ float max2_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float min_nan(float a, float b, float c) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-// One warp a (sequence, page, KV head), a lane eight channels of 16 / (32 / (D / 8)) tokens of
-// a tile: all the loads of a tile are in flight together.  Two tokens a step of the three-operand
-// minimum and maximum; rounding to T is monotone and comes once, at the end.
+// A CTA of four warps takes four tiles: a page of four, or two of two, four of one.  A lane holds
+// eight channels of 16 / (32 / (D / 8)) tokens of its warp's tile, all loaded at once; two tokens a
+// step of the three-operand minimum and maximum.  A page of more tiles is its warps' in turn.
+// Rounding to T is monotone and comes once, after the warps of a page have met.
+constexpr int kBoundWarps = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(128) key_bounds_kernel(const PagedInt4 p, const Divisor by_each) {
+__global__ void __launch_bounds__(32 * kBoundWarps) key_bounds_kernel(const PagedInt4 p, const Divisor by_each, int warps_each) {
   constexpr int W = D / kInt4Group, kWords = D / 8, kStep = 32 / kWords, kTokens = kInt4Tile / kStep;
+  __shared__ float s_low[kBoundWarps][8][kWords], s_high[kBoundWarps][8][kWords];
   release_dependents();
   dependency_wait();
-  const int lane = threadIdx.x % 32;
-  const uint32_t unit = blockIdx.x * 4 + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int part = warp % warps_each;  // of the page's warps
+  const uint32_t unit = blockIdx.x * (kBoundWarps / warps_each) + warp / warps_each;
   const uint32_t row = quotient(unit, by_each);
   const int2 at = row_place(p, row);
   const int i = unit - row * by_each.d, h = at.y;
-  if (at.x >= p.batch) return;
-  const int tokens = static_cast<int>(row_tokens(p, at.x, 0));
-  const int before = tokens > p.new_tokens ? tokens - p.new_tokens : 0;
-  const int n = quotient(before, p.by_page) + i;
-  const int left = tokens - n * p.page_size;
-  if (n >= p.table_width || left <= 0) return;
-  const int64_t page = page_id(p, at.x, 0, n);
-  if (page < 0 || page >= p.num_pages) {
-    if (lane == 0) atomicMax(p.status, kStatusBadPageId);
-    return;
+  int64_t page = -1;
+  int live = 0;
+  if (at.x < p.batch) {
+    const int tokens = static_cast<int>(row_tokens(p, at.x, 0));
+    const int before = tokens > p.new_tokens ? tokens - p.new_tokens : 0;
+    const int n = quotient(before, p.by_page) + i;
+    const int left = tokens - n * p.page_size;
+    if (n < p.table_width && left > 0) {
+      page = page_id(p, at.x, 0, n);
+      if (page >= 0 && page < p.num_pages) {
+        live = min(left, p.page_size);
+      } else if (lane == 0 && part == 0) {
+        atomicMax(p.status, kStatusBadPageId);
+      }
+    }
   }
-  const int live = min(left, p.page_size);
   const int word = lane % kWords, t = word / W, w = word % W, first = lane / kWords;
   float low[8], high[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) low[j] = INFINITY, high[j] = -INFINITY;
-  const uint8_t* tile = p.pool + (page * p.kv_heads + h) * (p.page_size / kInt4Tile) * int4_tile_bytes(D);
-  for (int begin = 0; begin < live; begin += kInt4Tile, tile += int4_tile_bytes(D)) {
+  const uint8_t* tile = p.pool + ((page * p.kv_heads + h) * (p.page_size / kInt4Tile) + part) * int4_tile_bytes(D);
+  for (int begin = part * kInt4Tile; begin < live; begin += warps_each * kInt4Tile, tile += warps_each * int4_tile_bytes(D)) {
     uint32_t codes[kTokens];
     T steps[kTokens], floors[kTokens];
-#pragma unroll
-    for (int k = 0; k < kTokens; ++k) {
-      // behind the last token: the first one of the tile again, which every tile here has
-      const int r = begin + first + kStep * k < live ? first + kStep * k : 0;
+    auto load = [&](int k, int r) {
       codes[k] = *reinterpret_cast<const uint32_t*>(tile + r * (D / 2) + 4 * word);
       const T* params = reinterpret_cast<const T*>(tile + 16 * D) + r * W + w;
       steps[k] = params[0], floors[k] = params[D / 2];
+    };
+    if (begin + kInt4Tile <= live) {
+#pragma unroll
+      for (int k = 0; k < kTokens; ++k) load(k, first + kStep * k);
+    } else {  // behind the last token: the first one of the tile again, which every tile here has
+#pragma unroll
+      for (int k = 0; k < kTokens; ++k) load(k, begin + first + kStep * k < live ? first + kStep * k : 0);
     }
 #pragma unroll
     for (int k = 0; k < kTokens; k += 2) {
@@ -148,7 +153,22 @@ __global__ void __launch_bounds__(128) key_bounds_kernel(const PagedInt4 p, cons
       low[j] = min_nan(low[j], a, a), high[j] = max_nan(high[j], z, z);
     }
   }
-  if (lane < kWords) {
+  if (warps_each > 1) {
+    if (lane < kWords) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s_low[warp][j][lane] = low[j], s_high[warp][j][lane] = high[j];
+    }
+    __syncthreads();
+    if (part != 0) return;
+    for (int k = 1; k < warps_each; ++k) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float a = s_low[warp + k][j][word], z = s_high[warp + k][j][word];
+        low[j] = min_nan(low[j], a, a), high[j] = max_nan(high[j], z, z);
+      }
+    }
+  }
+  if (live > 0 && lane < kWords) {
     T* dst = static_cast<T*>(p.bounds) + (page * p.kv_heads + h) * 2 * D + 32 * w + 8 * t;
     *reinterpret_cast<uint4*>(dst) =
         make_uint4(pack2<T>(low[0], low[1]), pack2<T>(low[2], low[3]), pack2<T>(low[4], low[5]), pack2<T>(low[6], low[7]));
@@ -164,33 +184,35 @@ __device__ __forceinline__ uint32_t score_key(float s) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// keys[row][n], row = b * kv_heads + h: D / 8 lanes a page, eight channels each, two pages a lane
-// in flight; the row's queries are held as floats in shared memory.
+// keys[row][n], row = b * kv_heads + h: D / 8 lanes a page, eight channels each, two pages a lane,
+// whose products and sums are the two halves of packed instructions; the row's queries lie in
+// shared memory, every element twice for that.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) page_score_kernel(const PagedInt4 p, uint32_t* keys) {
-  constexpr int kLanes = D / 8, kPages = 32 / kLanes, kMaxGroup = 16;
-  __shared__ __align__(16) float s_q[kMaxGroup][D];
+__global__ void __launch_bounds__(128) page_score_kernel(const PagedInt4 p, uint32_t* keys) {
+  constexpr int kLanes = D / 8, kPages = 32 / kLanes, kMaxGroup = 16, kCtaPages = 4 * 2 * kPages;
+  __shared__ __align__(16) float4 s_q[kMaxGroup][4][kLanes];  // two channels of a lane: neighbouring lanes, neighbouring banks
   release_dependents();
   dependency_wait();
   const int row = blockIdx.y;
   const int2 at = row_place(p, row);
   const int b = at.x, h = at.y;
   const int lane = threadIdx.x % 32, l = lane % kLanes;
+  const int group = p.q_heads / p.kv_heads;
   const int tokens = static_cast<int>(row_tokens(p, b, 0));
   const int count = quotient(tokens + p.page_size - 1, p.by_page);
-  const int warp_first = (blockIdx.x * 8 + threadIdx.x / 32) * 2 * kPages;
-  if (count <= p.take || blockIdx.x * 16 * kPages >= count - 1) return;  // every page is taken, or none is left
-  const int group = p.q_heads / p.kv_heads;
-  for (int i = threadIdx.x; i < group * (D / 8); i += 256) {
+  if (count <= p.take || static_cast<int>(blockIdx.x) * kCtaPages >= count - 1) return;  // every page is taken, or none is left
+  for (int i = threadIdx.x; i < group * (D / 8); i += 128) {
     const int g = i / (D / 8), d = i % (D / 8) * 8;
     const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_sb + static_cast<int64_t>(h * group + g) * p.q_sh + d);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(&s_q[g][d + 2 * j]) = unpack2<T>((&raw.x)[j]);
+    for (int j = 0; j < 4; ++j) {
+      const float2 x = unpack2<T>((&raw.x)[j]);
+      s_q[g][j][d / 8] = make_float4(x.x, x.x, x.y, x.y);
+    }
   }
   __syncthreads();
-  const int step = gridDim.x * 16 * kPages;
-  for (int first = warp_first; first < count - 1; first += step) {
-    float low[2][8], high[2][8];
+  for (int first = blockIdx.x * kCtaPages + threadIdx.x / 32 * 2 * kPages; first < count - 1; first += gridDim.x * kCtaPages) {
+    uint4 lo[2], hi[2];
     bool ok[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -198,38 +220,36 @@ __global__ void __launch_bounds__(256) page_score_kernel(const PagedInt4 p, uint
       const int64_t page = n < count - 1 ? page_id(p, b, 0, n) : -1;
       ok[k] = page >= 0 && page < p.num_pages;
       if (!ok[k] && n < count - 1 && l == 0) atomicMax(p.status, kStatusBadPageId);
-      uint4 a = make_uint4(0, 0, 0, 0), z = a;
+      lo[k] = hi[k] = make_uint4(0, 0, 0, 0);
       if (ok[k]) {
         const T* src = static_cast<const T*>(p.bounds) + (page * p.kv_heads + h) * 2 * D + 8 * l;
-        a = *reinterpret_cast<const uint4*>(src), z = *reinterpret_cast<const uint4*>(src + D);
+        lo[k] = *reinterpret_cast<const uint4*>(src), hi[k] = *reinterpret_cast<const uint4*>(src + D);
       }
+    }
+    uint64_t low[8], high[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 lo = unpack2<T>((&a.x)[j]), hi = unpack2<T>((&z.x)[j]);
-        low[k][2 * j] = lo.x, low[k][2 * j + 1] = lo.y, high[k][2 * j] = hi.x, high[k][2 * j + 1] = hi.y;
-      }
+    for (int j = 0; j < 4; ++j) {
+      const float2 a = unpack2<T>((&lo[0].x)[j]), c = unpack2<T>((&lo[1].x)[j]), y = unpack2<T>((&hi[0].x)[j]), z = unpack2<T>((&hi[1].x)[j]);
+      low[2 * j] = pair32(a.x, c.x), low[2 * j + 1] = pair32(a.y, c.y);
+      high[2 * j] = pair32(y.x, z.x), high[2 * j + 1] = pair32(y.y, z.y);
     }
     float best[2] = {-INFINITY, -INFINITY};
     for (int g = 0; g < group; ++g) {
-      float q[8];
-      *reinterpret_cast<float4*>(q) = *reinterpret_cast<const float4*>(&s_q[g][8 * l]);
-      *reinterpret_cast<float4*>(q + 4) = *reinterpret_cast<const float4*>(&s_q[g][8 * l + 4]);
-      float s[2];
+      uint64_t term[8];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float term[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) term[j] = max_nan(__fmul_rn(q[j], low[k][j]), __fmul_rn(q[j], high[k][j]));
-        s[k] = __fadd_rn(__fadd_rn(__fadd_rn(term[0], term[1]), __fadd_rn(term[2], term[3])),
-                         __fadd_rn(__fadd_rn(term[4], term[5]), __fadd_rn(term[6], term[7])));
+      for (int j = 0; j < 8; j += 2) {
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(&s_q[g][j / 2][l]);
+        const float2 a = unpair32(mul32x2(q.x, low[j])), c = unpair32(mul32x2(q.x, high[j]));
+        const float2 y = unpair32(mul32x2(q.y, low[j + 1])), z = unpair32(mul32x2(q.y, high[j + 1]));
+        term[j] = pair32(max2_nan(a.x, c.x), max2_nan(a.y, c.y));
+        term[j + 1] = pair32(max2_nan(y.x, z.x), max2_nan(y.y, z.y));
       }
+      uint64_t s = add32x2(add32x2(add32x2(term[0], term[1]), add32x2(term[2], term[3])),
+                           add32x2(add32x2(term[4], term[5]), add32x2(term[6], term[7])));
 #pragma unroll
-      for (int off = 1; off < kLanes; off <<= 1) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) s[k] = __fadd_rn(s[k], __shfl_xor_sync(0xffffffffu, s[k], off));
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) best[k] = max_nan(best[k], s[k]);
+      for (int off = 1; off < kLanes; off <<= 1) s = add32x2(s, __shfl_xor_sync(0xffffffffu, s, off));
+      const float2 both = unpair32(s);
+      best[0] = max2_nan(best[0], both.x), best[1] = max2_nan(best[1], both.y);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -293,9 +313,20 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const PagedInt4
       for (int n = first; n < end; ++n) f(n, mine[n]);
     }
   };
-  uint32_t least = 0;  // the largest value that at least `want` keys reach
+  // the largest value that at least `want` keys reach; the bits that all keys share are known
+  uint32_t low = 0xffffffffu, high = 0u;
+  visit([&](int n, uint32_t key) {
+    if (n < end) low = min(low, key), high = max(high, key);
+  });
+  low = __reduce_min_sync(0xffffffffu, low), high = __reduce_max_sync(0xffffffffu, high);
+  if (lane == 0) s_sum[1][0][warp] = static_cast<int>(low), s_sum[1][1][warp] = static_cast<int>(high);
+  __syncthreads();
+  low = __reduce_min_sync(0xffffffffu, lane < kPickThreads / 32 ? static_cast<uint32_t>(s_sum[1][0][lane]) : 0xffffffffu);
+  high = __reduce_max_sync(0xffffffffu, lane < kPickThreads / 32 ? static_cast<uint32_t>(s_sum[1][1][lane]) : 0u);
+  const int top = low == high ? -1 : (31 - __clz(low ^ high)) & ~1;  // lowest bit of the first pair that differs
+  uint32_t least = top < 0 ? low : top >= 30 ? 0u : high >> (top + 2) << (top + 2);
   int phase = 0;
-  for (int shift = 30; shift >= 0; shift -= 2, phase ^= 1) {
+  for (int shift = top; shift >= 0; shift -= 2, phase ^= 1) {
     const uint32_t one = least | (1u << shift), two = least | (2u << shift), three = least | (3u << shift);
     int a = 0, c = 0, e = 0;
     visit([&](int, uint32_t key) { a += key >= one, c += key >= two, e += key >= three; });
@@ -345,6 +376,7 @@ PagedInt4 over_selection(PagedInt4 p) {
   p.t_sb = static_cast<int64_t>(p.kv_heads) * p.take, p.t_sh = p.take, p.t_sp = 1;
   p.lens = p.page_lens, p.lens_dtype = QF_INDEX_I32;
   p.l_sb = p.kv_heads, p.l_sh = 1;
+  p.early = false;  // the kernel in front writes both
   return p;
 }
 
@@ -354,21 +386,23 @@ int launch_select(const PagedInt4& p, int head_dim, int dtype, cudaStream_t stre
   const int rows = p.batch * p.kv_heads;
   QF_REQUIRE(rows <= 65535, "at most 65535 (sequence, KV head) rows choose pages in one call");
   uint32_t* keys = static_cast<uint32_t*>(p.workspace);
-  const int64_t pages = head_dim == 128 ? 32 : 64;  // of a CTA at a time
+  const int64_t pages = head_dim == 128 ? 16 : 32;  // of a CTA at a time
   const int64_t blocks = (p.table_width + pages - 1) / pages;
   const dim3 grid(static_cast<unsigned>(blocks < 1 ? 1 : blocks > 2048 ? 2048 : blocks), rows);
   cudaError_t err = cudaSuccess;
   if (dtype == QF_DTYPE_F16) {
-    err = head_dim == 128 ? launch_chained(page_score_kernel<__half, 128>, grid, dim3(256), 0, stream, p, keys)
-                          : launch_chained(page_score_kernel<__half, 64>, grid, dim3(256), 0, stream, p, keys);
+    err = head_dim == 128 ? launch_chained(page_score_kernel<__half, 128>, grid, dim3(128), 0, stream, p, keys)
+                          : launch_chained(page_score_kernel<__half, 64>, grid, dim3(128), 0, stream, p, keys);
   } else {
-    err = head_dim == 128 ? launch_chained(page_score_kernel<__nv_bfloat16, 128>, grid, dim3(256), 0, stream, p, keys)
-                          : launch_chained(page_score_kernel<__nv_bfloat16, 64>, grid, dim3(256), 0, stream, p, keys);
+    err = head_dim == 128 ? launch_chained(page_score_kernel<__nv_bfloat16, 128>, grid, dim3(128), 0, stream, p, keys)
+                          : launch_chained(page_score_kernel<__nv_bfloat16, 64>, grid, dim3(128), 0, stream, p, keys);
   }
   QF_CUDA(err);
   const uint32_t* scored = keys;
   if (p.table_width <= 2 * kPickThreads) {
     err = launch_chained(page_pick_kernel<2>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored);
+  } else if (p.table_width <= 5 * kPickThreads) {
+    err = launch_chained(page_pick_kernel<5>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored);
   } else if (p.table_width <= 16 * kPickThreads) {
     err = launch_chained(page_pick_kernel<16>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored);
   } else {
@@ -395,16 +429,17 @@ int qf_int4_key_bounds(const qf_paged_int4_args* args, void* stream) {
   const int pages_each = static_cast<int>(spanned < p.table_width ? spanned : p.table_width);
   const int64_t units = static_cast<int64_t>(p.batch) * p.kv_heads * pages_each;
   QF_REQUIRE(units < (1LL << 31) - 4, "too many pages in one call");
-  const dim3 grid(static_cast<unsigned>((units + 3) / 4));
+  const int tiles = p.page_size / kInt4Tile, warps_each = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1, pages_a_cta = kBoundWarps / warps_each;
+  const dim3 grid(static_cast<unsigned>((units + pages_a_cta - 1) / pages_a_cta));
   const Divisor by_each = make_divisor(pages_each);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t err = cudaSuccess;
   if (args->dtype == QF_DTYPE_F16) {
-    err = args->head_dim == 128 ? launch_chained(key_bounds_kernel<__half, 128>, grid, dim3(128), 0, s, p, by_each)
-                                : launch_chained(key_bounds_kernel<__half, 64>, grid, dim3(128), 0, s, p, by_each);
+    err = args->head_dim == 128 ? launch_chained(key_bounds_kernel<__half, 128>, grid, dim3(32 * kBoundWarps), 0, s, p, by_each, warps_each)
+                                : launch_chained(key_bounds_kernel<__half, 64>, grid, dim3(32 * kBoundWarps), 0, s, p, by_each, warps_each);
   } else {
-    err = args->head_dim == 128 ? launch_chained(key_bounds_kernel<__nv_bfloat16, 128>, grid, dim3(128), 0, s, p, by_each)
-                                : launch_chained(key_bounds_kernel<__nv_bfloat16, 64>, grid, dim3(128), 0, s, p, by_each);
+    err = args->head_dim == 128 ? launch_chained(key_bounds_kernel<__nv_bfloat16, 128>, grid, dim3(32 * kBoundWarps), 0, s, p, by_each, warps_each)
+                                : launch_chained(key_bounds_kernel<__nv_bfloat16, 64>, grid, dim3(32 * kBoundWarps), 0, s, p, by_each, warps_each);
   }
   QF_CUDA(err);
   QF_CUDA(cudaGetLastError());
@@ -424,9 +459,6 @@ int qf_int4_sparse_decode_attention(const qf_paged_int4_args* args, void* stream
   using namespace qf;
   PagedInt4 p;
   if (const int rc = fill_paged_int4(args, kNeedsQuery | kNeedsPool | kNeedsOut | kNeedsBounds | kNeedsSelection, &p)) return rc;
-  QF_REQUIRE(p.take < (1LL << 30) / p.page_size, "the pages taken hold 2^30 tokens or more");
-  QF_REQUIRE(static_cast<int64_t>(p.batch) * p.kv_heads * p.take < (1LL << 30) / (p.page_size / kInt4Tile),
-             "the pages taken hold 2^30 tiles of 16 tokens or more");
   if (p.batch == 0) return QF_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   PagedInt4 next = over_selection(p);

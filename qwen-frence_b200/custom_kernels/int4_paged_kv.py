@@ -34,6 +34,8 @@ import importlib.util
 import sys
 from pathlib import Path
 
+import torch
+
 TILE_TOKENS = 16
 MAX_GROUP = 16
 
@@ -60,36 +62,53 @@ def _require(condition, message):
         raise ValueError(message)
 
 
-def _check_pool(torch, pool):
-    """(kv_heads, head_dim, page_size) of a 4-bit pool."""
-    _require(pool.ndim == 4 and pool.dtype == torch.uint8 and pool.shape[3] in (1280, 2560),
-             "a 4-bit pool is uint8 [pages, kv_heads, page_size / 16, 20 * head_dim] with head_dim 64 or 128")
-    _require(pool.shape[1] >= 1 and pool.shape[2] >= 1, "a 4-bit pool has at least one KV head and one tile a page")
-    _require(pool.is_cuda, "the 4-bit cache needs a CUDA device")
-    _require(pool.is_contiguous() and pool.data_ptr() % 16 == 0, "a 4-bit pool must be contiguous and 16-byte aligned")
-    return pool.shape[1], pool.shape[3] // 20, pool.shape[2] * TILE_TOKENS
+_ELEMENT_CODES = {torch.float16: 0, torch.bfloat16: 1}
+_INDEX_CODES = {torch.int32: 0, torch.int64: 1}
 
 
-def _element_code(torch, dtype):
-    if dtype is torch.float16:
-        return 0
-    if dtype is torch.bfloat16:
-        return 1
-    raise ValueError("a 4-bit cache is written and read as float16 or bfloat16")
+def _check_pool(pool):
+    """(pages, kv_heads, head_dim, page_size) of a 4-bit pool."""
+    shape = pool.shape
+    if len(shape) != 4 or pool.dtype is not torch.uint8 or shape[3] not in (1280, 2560):
+        raise ValueError("a 4-bit pool is uint8 [pages, kv_heads, page_size / 16, 20 * head_dim] with head_dim 64 or 128")
+    pages, kv_heads, tiles, width = shape
+    if kv_heads < 1 or tiles < 1:
+        raise ValueError("a 4-bit pool has at least one KV head and one tile a page")
+    if not pool.is_cuda:
+        raise ValueError("the 4-bit cache needs a CUDA device")
+    if not pool.is_contiguous() or pool.data_ptr() % 16:
+        raise ValueError("a 4-bit pool must be contiguous and 16-byte aligned")
+    return pages, kv_heads, width // 20, tiles * TILE_TOKENS
 
 
-def _index_code(torch, tensor, what):
-    if tensor.dtype is torch.int32:
-        return 0
-    if tensor.dtype is torch.int64:
-        return 1
-    raise ValueError(f"{what} must use an integer dtype")
+def _element_code(dtype):
+    code = _ELEMENT_CODES.get(dtype)
+    if code is None:
+        raise ValueError("a 4-bit cache is written and read as float16 or bfloat16")
+    return code
+
+
+def _index_code(tensor, what):
+    code = _INDEX_CODES.get(tensor.dtype)
+    if code is None:
+        raise ValueError(f"{what} must use an integer dtype")
+    return code
+
+
+def _enqueue(function, *arguments, device):
+    """One library call on the current stream of CUDA device number `device`, which is current meanwhile."""
+    cabi = _cabi()
+    if torch.cuda.current_device() == device:
+        status = function(*arguments, cabi.raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = function(*arguments, cabi.raw_stream(device))
+    if status:
+        cabi.check(status)
 
 
 def empty_kv_pool_int4(num_pages, kv_heads, head_dim, *, page_size=16, device=None):
     """An uninitialised 4-bit pool for K and V; its rows are defined once they are written."""
-    import torch
-
     _require(head_dim in (64, 128), "head_dim must be 64 or 128")
     _require(page_size >= TILE_TOKENS and page_size % TILE_TOKENS == 0, "page_size must be a multiple of 16")
     return torch.empty((num_pages, kv_heads, page_size // TILE_TOKENS, 20 * head_dim), dtype=torch.uint8,
@@ -98,49 +117,50 @@ def empty_kv_pool_int4(num_pages, kv_heads, head_dim, *, page_size=16, device=No
 
 def empty_key_bounds_int4(kv4_pool, dtype):
     """Storage for the smallest and the largest key of every page: [pages, kv_heads, 2, D]."""
-    import torch
-
-    kv_heads, dim, _ = _check_pool(torch, kv4_pool)
-    _element_code(torch, dtype)
+    _, kv_heads, dim, _ = _check_pool(kv4_pool)
+    _element_code(dtype)
     return torch.empty((kv4_pool.shape[0], kv_heads, 2, dim), dtype=dtype, device=kv4_pool.device)
 
 
-def _write(q, k, v, q_out, q_strides, k_strides, v_strides, o_strides, positions, slot_mapping, pool, *,
-           rows, q_heads, kv_heads, head_dim, page_size, base, rope_table, valid_tokens=None):
-    """Check what every write shares, fill qf_int4_write_args and enqueue on the current stream."""
-    import torch
-
+def _write(pool, geometry, pointers, strides, like, positions, slot_mapping, *, rows, q_heads, base, rope_table,
+           valid_tokens=None):
+    """Check what every write shares, fill qf_int4_write_args and enqueue on the current stream.
+    `pointers` of q, k, v and q_out; `strides` of their rows, heads and channels, twelve numbers."""
+    pages, kv_heads, dim, page_size = geometry
     cabi = _cabi()
-    device = pool.device
-    dtype = _element_code(torch, k.dtype)
-    _require(v.dtype == k.dtype and (q is None or q.dtype == k.dtype), "Q/K/V must share FP16 or BF16 dtype")
-    operands = [t for t in (q, k, v, positions, slot_mapping, rope_table, valid_tokens) if t is not None]
-    _require(all(t.device == device for t in operands), "the 4-bit cache write needs CUDA tensors of one device")
-    positions_code = 0
+    device = pool.get_device()
+    dtype = _element_code(like.dtype)
+    _require(like.get_device() == device, "the 4-bit cache write needs CUDA tensors of one device")
+    position_at = position_stride = position_code = 0
     if positions is not None:
+        _require(positions.get_device() == device, "the 4-bit cache write needs CUDA tensors of one device")
         if positions.dtype is torch.float32 and rope_table is None:
-            positions_code = cabi.INDEX_F32
+            position_code = cabi.INDEX_F32
         else:
-            positions_code = _index_code(torch, positions, "positions")
+            position_code = _index_code(positions, "positions")
+        position_at, position_stride = positions.data_ptr(), positions.stride(0)
+    slot_at = slot_stride = slot_code = 0
+    if slot_mapping is not None:
+        _require(slot_mapping.get_device() == device, "the 4-bit cache write needs CUDA tensors of one device")
+        slot_at, slot_stride = slot_mapping.data_ptr(), slot_mapping.stride(0)
+        slot_code = _index_code(slot_mapping, "slot mapping")
+    table_at = table_positions = 0
     if rope_table is not None:
-        _require(rope_table.ndim == 3 and rope_table.shape[0] >= 1 and tuple(rope_table.shape[1:]) == (head_dim // 2, 2)
-                 and rope_table.dtype == torch.float32 and rope_table.is_contiguous(),
-                 "rope_table must be contiguous float32 [positions, head_dim / 2, 2]")
+        table_positions = rope_table.shape[0]
+        _require(rope_table.shape == (table_positions, dim // 2, 2) and table_positions >= 1
+                 and rope_table.dtype is torch.float32 and rope_table.is_contiguous() and rope_table.data_ptr() % 16 == 0,
+                 "rope_table must be contiguous, 16-byte aligned float32 [positions, head_dim / 2, 2]")
+        _require(rope_table.get_device() == device, "the 4-bit cache write needs CUDA tensors of one device")
+        table_at = rope_table.data_ptr()
+    valid_at = None
     if valid_tokens is not None:
-        _require(valid_tokens.dtype == torch.int32 and valid_tokens.numel() == 1,
+        _require(valid_tokens.dtype is torch.int32 and valid_tokens.numel() == 1 and valid_tokens.get_device() == device,
                  "valid_tokens must be a CUDA int32 scalar")
+        valid_at = valid_tokens.data_ptr()
     args = cabi.Int4WriteArgs(
-        None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), None if q is None else q_out.data_ptr(),
-        *q_strides, *k_strides, *v_strides, *o_strides,
-        None if positions is None else positions.data_ptr(), 0 if positions is None else positions.stride(0),
-        None if slot_mapping is None else slot_mapping.data_ptr(), 0 if slot_mapping is None else slot_mapping.stride(0),
-        None if rope_table is None else rope_table.data_ptr(), pool.data_ptr(), pool.shape[0],
-        None if valid_tokens is None else valid_tokens.data_ptr(),
-        rows, q_heads, kv_heads, head_dim, page_size, dtype, positions_code,
-        0 if slot_mapping is None else _index_code(torch, slot_mapping, "slot mapping"),
-        0 if rope_table is None else rope_table.shape[0], float(base))
-    with cabi.device_of(pool):
-        cabi.check(cabi.library().qf_int4_rope_kv_write(ctypes.byref(args), cabi.stream_pointer(device)))
+        *pointers, *strides, position_at, position_stride, slot_at, slot_stride, table_at, pool.data_ptr(), pages, valid_at,
+        rows, q_heads, kv_heads, dim, page_size, dtype, position_code, slot_code, table_positions, base)
+    _enqueue(cabi.library().qf_int4_rope_kv_write, ctypes.byref(args), device=device)
 
 
 def packed_qkv_rope_cache_int4(
@@ -152,12 +172,10 @@ def packed_qkv_rope_cache_int4(
     row is skipped).  rope_table (positions, D / 2, 2) float32 (cos, sin) pairs; without it the
     angles are position * base^(-2i / D).  Rows at or beyond valid_tokens get zero queries and no
     cache write.  No two rows of a call may have the same slot."""
-    import torch
-
     if packed.ndim == 3:
         _require(packed.shape[1] == 1, "packed QKV must have one decode token per row")
         packed = packed[:, 0, :]
-    kv_heads, dim, page_size = _check_pool(torch, kv4_pool)
+    geometry = _, kv_heads, dim, _ = _check_pool(kv4_pool)
     _require(q_heads >= 1, "q_heads must be positive")
     _require(packed.ndim == 2 and packed.shape[1] == (q_heads + 2 * kv_heads) * dim,
              "expected packed QKV shape (rows, (q_heads + 2 * kv_heads) * head_dim)")
@@ -165,12 +183,27 @@ def packed_qkv_rope_cache_int4(
     _require(positions.shape == (rows,) and slot_mapping.shape == (rows,),
              "positions and slots must contain one value per row")
     q = torch.empty((rows, q_heads, dim), device=packed.device, dtype=packed.dtype)
+    if rows == 0:
+        return q
     row_stride, col_stride = packed.stride()
     segment = (row_stride, dim * col_stride, col_stride)
-    _write(packed, packed[:, q_heads * dim:], packed[:, (q_heads + kv_heads) * dim:], q, segment, segment, segment,
-           q.stride(), positions, slot_mapping, kv4_pool, rows=rows, q_heads=q_heads, kv_heads=kv_heads, head_dim=dim,
-           page_size=page_size, base=base, rope_table=rope_table, valid_tokens=valid_tokens)
+    at, head = packed.data_ptr(), 2 * dim * col_stride  # bytes from one head to the next
+    _write(kv4_pool, geometry, (at, at + q_heads * head, at + (q_heads + kv_heads) * head, q.data_ptr()),
+           (*segment, *segment, *segment, q_heads * dim, dim, 1), packed, positions, slot_mapping, rows=rows,
+           q_heads=q_heads, base=base, rope_table=rope_table, valid_tokens=valid_tokens)
     return q
+
+
+def _write_heads(q, k, v, positions, slot_mapping, kv4_pool, geometry, token_dim, rotate_q, base, rope_table):
+    """The write of tensors whose tokens lie along `token_dim` and heads along dimension 1."""
+    _require(k.dtype == v.dtype == q.dtype, "Q/K/V must share FP16 or BF16 dtype")
+    _require(q.get_device() == k.get_device() == v.get_device(), "the 4-bit cache write needs CUDA tensors of one device")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if rotate_q else q
+    strides = tuple(t.stride(n) for t in (q, k, v, out) for n in (token_dim, 1, 3))
+    _write(kv4_pool, geometry, (q.data_ptr() if rotate_q else None, k.data_ptr(), v.data_ptr(), out.data_ptr() if rotate_q else None),
+           strides, k, positions, slot_mapping, rows=k.shape[token_dim], q_heads=q.shape[1] if rotate_q else 0, base=base,
+           rope_table=rope_table)
+    return out
 
 
 def native_decode_rope_kv_write_int4(
@@ -178,140 +211,137 @@ def native_decode_rope_kv_write_int4(
 ):
     """native_decode_rope_kv_write for the 4-bit cache: q (B, Hq, 1, D), k and v (B, Hkv, 1, D).
     Returns rotated Q (or q when rotate_q=False)."""
-    import torch
-
     _require(all(t.ndim == 4 and t.shape[2] == 1 for t in (q, k, v)),
              "decode Q/K/V must have shape (batch, heads, 1, dim)")
-    kv_heads, dim, page_size = _check_pool(torch, kv4_pool)
+    geometry = _, kv_heads, dim, _ = _check_pool(kv4_pool)
     batch = q.shape[0]
-    _require(k.shape == v.shape and tuple(k.shape) == (batch, kv_heads, 1, dim) and q.shape[-1] == dim,
+    _require(k.shape == v.shape and k.shape == (batch, kv_heads, 1, dim) and q.shape[-1] == dim,
              "decode K/V shapes do not match Q and the pool")
     _require(positions.shape == (batch,) and slot_mapping.shape == (batch,),
              "positions and slots must contain one entry per batch row")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if rotate_q else q
-    rows_of = lambda t: (t.stride(0), t.stride(1), t.stride(3))  # noqa: E731
-    _write(q if rotate_q else None, k, v, out, rows_of(q), rows_of(k), rows_of(v), rows_of(out), positions, slot_mapping,
-           kv4_pool, rows=batch, q_heads=q.shape[1] if rotate_q else 0, kv_heads=kv_heads, head_dim=dim,
-           page_size=page_size, base=base, rope_table=rope_table)
-    return out
+    return _write_heads(q, k, v, positions, slot_mapping, kv4_pool, geometry, 0, rotate_q, base, rope_table)
 
 
 def rope_kv_write_int4(q, k, v, positions, slot_mapping, kv4_pool, *, base=1_000_000.0, rope_table=None):
     """rope_kv_write for the 4-bit cache: q (1, Hq, T, D), k and v (1, Hkv, T, D), one prompt or a
     packed chunk of several.  Returns rotated Q shaped like q."""
-    import torch
-
     _require(q.ndim == 4 and k.ndim == 4 and v.ndim == 4, "q, k, and v must be rank-four tensors")
     _require(q.shape[0] == 1 and k.shape[0] == 1 and v.shape[0] == 1,
              "packed q, k, and v must have batch dimension one")
-    kv_heads, dim, page_size = _check_pool(torch, kv4_pool)
+    geometry = _, kv_heads, dim, _ = _check_pool(kv4_pool)
     tokens = q.shape[2]
-    _require(k.shape == v.shape and tuple(k.shape) == (1, kv_heads, tokens, dim) and q.shape[-1] == dim,
+    _require(k.shape == v.shape and k.shape == (1, kv_heads, tokens, dim) and q.shape[-1] == dim,
              "K/V shapes do not match Q and the pool")
     if positions.ndim == 2:
         _require(tuple(positions.shape) == (1, tokens), "positions must have shape (1, tokens)")
         positions = positions[0]
     _require(positions.shape == (tokens,) and slot_mapping.shape == (tokens,),
              "positions and slots must contain one entry per token")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    rows_of = lambda t: (t.stride(2), t.stride(1), t.stride(3))  # noqa: E731
-    _write(q, k, v, out, rows_of(q), rows_of(k), rows_of(v), rows_of(out), positions, slot_mapping, kv4_pool,
-           rows=tokens, q_heads=q.shape[1], kv_heads=kv_heads, head_dim=dim, page_size=page_size, base=base,
-           rope_table=rope_table)
-    return out
+    return _write_heads(q, k, v, positions, slot_mapping, kv4_pool, geometry, 2, True, base, rope_table)
 
 
 def quantize_kv_pool_int4(k_pool, v_pool):
     """A 4-bit pool with the contents of fp16 / bf16 pools [pages, page_size, Hkv, D] (keys as they are:
     already rotated).  Every row of the pools is quantised; rows with a NaN or an infinity read back as NaN."""
-    import torch
-
     _require(k_pool.ndim == 4 and k_pool.shape == v_pool.shape and k_pool.is_contiguous() and v_pool.is_contiguous(),
              "K/V pools must be contiguous with matching rank-four shapes")
     pages, page_size, kv_heads, dim = k_pool.shape
     _require(k_pool.is_cuda and v_pool.device == k_pool.device, "K/V pools must share one CUDA device")
     pool = empty_kv_pool_int4(pages, kv_heads, dim, page_size=page_size, device=k_pool.device)
-    strides = (kv_heads * dim, dim, 1)
-    _write(None, k_pool, v_pool, None, strides, strides, strides, strides, None, None, pool, rows=pages * page_size,
-           q_heads=0, kv_heads=kv_heads, head_dim=dim, page_size=page_size, base=1.0, rope_table=None)
+    _require(v_pool.dtype == k_pool.dtype, "K/V pools must share FP16 or BF16 dtype")
+    _write(pool, (pages, kv_heads, dim, page_size), (None, k_pool.data_ptr(), v_pool.data_ptr(), None),
+           (kv_heads * dim, dim, 1) * 4, k_pool, None, None, rows=pages * page_size, q_heads=0, base=1.0, rope_table=None)
     return pool
 
 
-def _read(torch, kv4_pool, slot_mapping, rows, dtype):
-    cabi = _cabi()
-    kv_heads, dim, page_size = _check_pool(torch, kv4_pool)
-    code = _element_code(torch, dtype)
-    k = torch.empty((rows, kv_heads, dim), dtype=dtype, device=kv4_pool.device)
-    v = torch.empty((rows, kv_heads, dim), dtype=dtype, device=kv4_pool.device)
-    slots = (None, 0, 0)
-    if slot_mapping is not None:
-        slots = (slot_mapping.data_ptr(), _index_code(torch, slot_mapping, "slot mapping"), slot_mapping.stride(0))
-    with cabi.device_of(kv4_pool):
-        cabi.check(cabi.library().qf_int4_read_rows(
-            kv4_pool.data_ptr(), kv4_pool.shape[0], page_size, kv_heads, dim, code, *slots, rows, k.data_ptr(),
-            v.data_ptr(), cabi.stream_pointer(kv4_pool.device)))
-    return k, v
+def _read(kv4_pool, slots, rows, dtype):
+    """Rows at `slots` = (address, index code, stride) as K and V [rows, kv_heads, D]."""
+    pages, kv_heads, dim, page_size = _check_pool(kv4_pool)
+    code = _element_code(dtype)
+    both = torch.empty((2, rows, kv_heads, dim), dtype=dtype, device=kv4_pool.device)
+    at = both.data_ptr()
+    _enqueue(_cabi().library().qf_int4_read_rows, kv4_pool.data_ptr(), pages, page_size, kv_heads, dim, code, *slots, rows,
+             at, at + 2 * rows * kv_heads * dim, device=kv4_pool.get_device())
+    return both.unbind(0)
 
 
 def read_kv_int4(kv4_pool, slot_mapping, *, dtype=None):
     """Rows of the cache at a list of slots as (k, v), both [n, Hkv, D] in `dtype` (that of the
     writes; default float16).  A slot outside the pool, -1 for one, gives a row of zeros."""
-    import torch
-
     _require(slot_mapping.ndim == 1, "slot mapping must be a list of slots")
-    _require(slot_mapping.device == kv4_pool.device, "pool and slots must share one CUDA device")
-    return _read(torch, kv4_pool, slot_mapping, slot_mapping.shape[0], torch.float16 if dtype is None else dtype)
+    _require(slot_mapping.get_device() == kv4_pool.get_device(), "pool and slots must share one CUDA device")
+    slots = (slot_mapping.data_ptr(), _index_code(slot_mapping, "slot mapping"), slot_mapping.stride(0))
+    return _read(kv4_pool, slots, slot_mapping.shape[0], torch.float16 if dtype is None else dtype)
 
 
 def dequantize_kv_pool_int4(kv4_pool, dtype=None):
     """The whole cache as 16-bit pools (k_pool, v_pool), both [pages, page_size, Hkv, D]."""
-    import torch
-
-    kv_heads, dim, page_size = _check_pool(torch, kv4_pool)
-    k, v = _read(torch, kv4_pool, None, kv4_pool.shape[0] * page_size, torch.float16 if dtype is None else dtype)
-    shape = (kv4_pool.shape[0], page_size, kv_heads, dim)
+    pages, kv_heads, dim, page_size = _check_pool(kv4_pool)
+    k, v = _read(kv4_pool, (None, 0, 0), pages * page_size, torch.float16 if dtype is None else dtype)
+    shape = (pages, page_size, kv_heads, dim)
     return k.view(shape), v.view(shape)
 
 
-def _paged(torch, cabi, batch, kv_heads, dim, page_size, num_pages, dtype, block_table, seq_lens, *, per_head,
-           q=None, out=None, pool=None, bounds=None, page_table=None, page_lens=None, new_tokens=0, take=0, scale=0.0):
-    """Check table and lengths and fill qf_paged_int4_args (no workspace yet)."""
-    heads_too = per_head and block_table.ndim == 3
-    if heads_too:
-        _require(tuple(block_table.shape[:2]) == (batch, kv_heads) and tuple(seq_lens.shape) == (batch, kv_heads),
+# scratch bytes by call, device and sizes: what qf_paged_int4_workspace answers is a function of these
+_workspace_sizes = {}
+
+_PAGED_DEVICE = "queries, pool, key bounds, page table and lengths must share one CUDA device"
+
+
+def _paged(device, batch, geometry, dtype, block_table, seq_lens, *, q=None, out=None, pool=None, bounds=None, choice=None,
+           new_tokens=0, take=0, scale=0.0, call=None):
+    """Check table and lengths, fill qf_paged_int4_args and add the scratch of `call`: a torch
+    allocation, so it is the stream's, and a captured graph's own.  Returns (args, scratch)."""
+    pages, kv_heads, dim, page_size = geometry
+    cabi = _cabi()
+    t_shape, l_shape = block_table.shape, seq_lens.shape
+    if len(t_shape) == 3 and call == cabi.INT4_ATTENTION:
+        _require(t_shape[:2] == (batch, kv_heads) and l_shape == (batch, kv_heads),
                  "a table and lengths per KV head have shapes [batch, kv_heads, pages] and [batch, kv_heads]")
-        t_sb, t_sh, t_sp = block_table.stride()
-        l_sb, l_sh = seq_lens.stride()
+        t_strides, l_strides = block_table.stride(), seq_lens.stride()
     else:
-        _require(block_table.ndim == 2 and seq_lens.ndim == 1 and block_table.shape[0] == batch
-                 and seq_lens.shape[0] == batch, "batch dimensions must match")
-        (t_sb, t_sp), t_sh = block_table.stride(), 0
-        l_sb, l_sh = seq_lens.stride(0), 0
-    q_strides = (0, 0) if q is None else (q.stride(0), q.stride(1))
-    o_strides = (0, 0) if out is None else (out.stride(0), out.stride(1))
-    pointer = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    return cabi.PagedInt4Args(
-        pointer(q), pointer(out), pointer(pool), pointer(bounds), block_table.data_ptr(), seq_lens.data_ptr(), None,
-        pointer(page_table), pointer(page_lens), *q_strides, *o_strides, t_sb, t_sh, t_sp, l_sb, l_sh,
-        num_pages, block_table.shape[-1], 0, batch, 0 if q is None else q.shape[1], kv_heads, dim, page_size, dtype,
-        _index_code(torch, block_table, "page table"), _index_code(torch, seq_lens, "lengths"), new_tokens, take, scale)
+        _require(len(t_shape) == 2 and t_shape[0] == batch and l_shape == (batch,), "batch dimensions must match")
+        t_strides, l_strides = (block_table.stride(0), 0, block_table.stride(1)), (seq_lens.stride(0), 0)
+    _require(block_table.get_device() == device and seq_lens.get_device() == device, _PAGED_DEVICE)
+    q_at = o_at = pages_at = held_at = None
+    q_heads = q_sb = q_sh = o_sb = o_sh = 0
+    if q is not None:
+        q_at, q_heads = q.data_ptr(), q.shape[1]
+        q_sb, q_sh, _ = q.stride()
+    if out is not None:
+        o_at, o_sb, o_sh = out.data_ptr(), q_heads * dim, dim
+    if choice is not None:
+        pages_at, held_at = choice[0].data_ptr(), choice[1].data_ptr()
+    args = cabi.PagedInt4Args(
+        q_at, o_at, None if pool is None else pool.data_ptr(), None if bounds is None else bounds.data_ptr(),
+        block_table.data_ptr(), seq_lens.data_ptr(), None, pages_at, held_at, q_sb, q_sh, o_sb, o_sh, *t_strides, *l_strides,
+        pages, t_shape[-1], 0, batch, q_heads, kv_heads, dim, page_size, dtype, _index_code(block_table, "page table"),
+        _index_code(seq_lens, "lengths"), new_tokens, take, scale)
+    scratch = None
+    if call is not None:
+        key = (call, device, batch, q_heads, kv_heads, dim, page_size, t_shape[-1], take)
+        need = _workspace_sizes.get(key)
+        if need is None:
+            size = ctypes.c_int64()
+            with torch.cuda.device(device):
+                cabi.check(cabi.library().qf_paged_int4_workspace(ctypes.byref(args), call, ctypes.byref(size)))
+            if len(_workspace_sizes) >= 4096:
+                _workspace_sizes.clear()
+            need = _workspace_sizes[key] = size.value
+        scratch = torch.empty(need, dtype=torch.uint8, device=block_table.device)
+        args.workspace, args.workspace_bytes = scratch.data_ptr(), need
+    return args, scratch
 
 
-def _add_workspace(torch, cabi, args, call, device):
-    """Scratch of one call: a torch allocation, so it is the stream's (and a captured graph's own)."""
-    need = ctypes.c_int64(0)
-    cabi.check(cabi.library().qf_paged_int4_workspace(ctypes.byref(args), call, ctypes.byref(need)))
-    scratch = torch.empty(need.value, dtype=torch.uint8, device=device)
-    args.workspace, args.workspace_bytes = scratch.data_ptr(), need.value
-    return scratch
-
-
-def _check_query(torch, q, kv_heads, dim):
+def _check_query(q, geometry):
     """q as the kernels take it: unit inner stride, rows on 16-byte boundaries."""
-    _require(q.ndim == 3 and q.shape[1] >= 1 and q.shape[2] == dim, "q must have shape [batch, query_heads, head_dim]")
-    _require(q.shape[1] % kv_heads == 0, "query heads must be divisible by KV heads")
-    _require(q.shape[1] // kv_heads <= MAX_GROUP, "at most 16 query heads share a KV head")
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    _, kv_heads, dim, _ = geometry
+    shape = q.shape
+    _require(len(shape) == 3 and shape[1] >= 1 and shape[2] == dim, "q must have shape [batch, query_heads, head_dim]")
+    _require(shape[1] % kv_heads == 0, "query heads must be divisible by KV heads")
+    _require(shape[1] // kv_heads <= MAX_GROUP, "at most 16 query heads share a KV head")
+    row, head, inner = q.stride()
+    if inner != 1 or row % 8 or head % 8 or q.data_ptr() % 16:
         q = q.contiguous()
         q = q.clone() if q.data_ptr() % 16 else q
     return q
@@ -325,30 +355,28 @@ def paged_decode_attention_int4(q, kv4_pool, block_table, seq_lens, *, scale=Non
     (what select_kv_pages returns).  seq_lens counts the tokens attended, the newest included; a row of
     length 0 gives zeros.  Default scale D ** -0.5.  The split over the GPU is planned on the device from
     the lengths, so there is no split_k."""
-    import torch
-
+    geometry = _check_pool(kv4_pool)
+    dtype = _element_code(q.dtype)
+    q = _check_query(q, geometry)
+    device = kv4_pool.get_device()
+    _require(q.get_device() == device, _PAGED_DEVICE)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     cabi = _cabi()
-    kv_heads, dim, page_size = _check_pool(torch, kv4_pool)
-    dtype = _element_code(torch, q.dtype)
-    q = _check_query(torch, q, kv_heads, dim)
-    device = kv4_pool.device
-    _require(q.device == device and block_table.device == device and seq_lens.device == device,
-             "q, pool, page table and lengths must share one CUDA device")
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    args = _paged(torch, cabi, q.shape[0], kv_heads, dim, page_size, kv4_pool.shape[0], dtype, block_table, seq_lens,
-                  per_head=True, q=q, out=out, pool=kv4_pool, scale=dim ** -0.5 if scale is None else scale)
-    with cabi.device_of(kv4_pool):
-        scratch = _add_workspace(torch, cabi, args, cabi.INT4_ATTENTION, device)
-        cabi.check(cabi.library().qf_int4_decode_attention(ctypes.byref(args), cabi.stream_pointer(device)))
+    args, scratch = _paged(device, q.shape[0], geometry, dtype, block_table, seq_lens, q=q, out=out, pool=kv4_pool,
+                           scale=geometry[2] ** -0.5 if scale is None else scale, call=cabi.INT4_ATTENTION)
+    _enqueue(cabi.library().qf_int4_decode_attention, ctypes.byref(args), device=device)
     del scratch
     return out
 
 
-def _check_bounds(torch, bounds, dtype):
-    _require(bounds.ndim == 4 and bounds.shape[2] == 2 and bounds.shape[3] in (64, 128) and bounds.dtype == dtype
-             and bounds.is_contiguous() and bounds.data_ptr() % 16 == 0,
+def _check_bounds(bounds, dtype, geometry=None):
+    """Key bounds of a pool's geometry (default: any)."""
+    shape = bounds.shape
+    _require(len(shape) == 4 and shape[2] == 2 and shape[3] in (64, 128) and bounds.dtype == dtype and bounds.is_contiguous()
+             and bounds.data_ptr() % 16 == 0,
              "key bounds must be contiguous [pages, kv_heads, 2, head_dim] in the queries' dtype")
     _require(bounds.is_cuda, "key bounds must be on a CUDA device")
+    _require(geometry is None or (shape[0], shape[1], shape[3]) == geometry[:3], "key bounds do not match the pool")
 
 
 def update_key_bounds_int4(kv4_pool, key_bounds, block_table, seq_lens, *, new_tokens=1):
@@ -357,29 +385,27 @@ def update_key_bounds_int4(kv4_pool, key_bounds, block_table, seq_lens, *, new_t
 
     Bounds are the smallest and the largest key of a page's tokens below seq_lens, per channel, as the
     cache reads back."""
-    import torch
-
-    cabi = _cabi()
-    kv_heads, dim, page_size = _check_pool(torch, kv4_pool)
-    dtype = _element_code(torch, key_bounds.dtype)
-    _check_bounds(torch, key_bounds, key_bounds.dtype)
-    _require(key_bounds.shape[0] == kv4_pool.shape[0] and key_bounds.shape[1] == kv_heads and key_bounds.shape[3] == dim,
-             "key bounds do not match the pool")
+    geometry = _check_pool(kv4_pool)
+    dtype = _element_code(key_bounds.dtype)
+    _check_bounds(key_bounds, key_bounds.dtype, geometry)
     _require(isinstance(new_tokens, int) and not isinstance(new_tokens, bool) and 0 <= new_tokens < 2 ** 31,
              "new_tokens must be a non-negative integer")
-    device = kv4_pool.device
-    _require(key_bounds.device == device and block_table.device == device and seq_lens.device == device,
-             "pool, key bounds, page table and lengths must share one CUDA device")
-    args = _paged(torch, cabi, block_table.shape[0], kv_heads, dim, page_size, kv4_pool.shape[0], dtype, block_table,
-                  seq_lens, per_head=False, pool=kv4_pool, bounds=key_bounds, new_tokens=new_tokens)
-    with cabi.device_of(kv4_pool):
-        cabi.check(cabi.library().qf_int4_key_bounds(ctypes.byref(args), cabi.stream_pointer(device)))
+    device = kv4_pool.get_device()
+    _require(key_bounds.get_device() == device, _PAGED_DEVICE)
+    args, _ = _paged(device, block_table.shape[0], geometry, dtype, block_table, seq_lens, pool=kv4_pool, bounds=key_bounds,
+                     new_tokens=new_tokens)
+    _enqueue(_cabi().library().qf_int4_key_bounds, ctypes.byref(args), device=device)
     return key_bounds
 
 
 def _check_take(num_pages):
     _require(isinstance(num_pages, int) and not isinstance(num_pages, bool) and 1 <= num_pages < 2 ** 31,
              "num_pages must be a positive integer")
+
+
+def _empty_choice(batch, kv_heads, num_pages, device):
+    return (torch.empty((batch, kv_heads, num_pages), dtype=torch.int32, device=device),
+            torch.empty((batch, kv_heads), dtype=torch.int32, device=device))
 
 
 def select_kv_pages(q, key_bounds, block_table, seq_lens, *, num_pages, page_size=16):
@@ -389,55 +415,40 @@ def select_kv_pages(q, key_bounds, block_table, seq_lens, *, num_pages, page_siz
     A row is the sequence's newest page and the num_pages - 1 others with the highest bound on a score,
     the largest over the KV head's query heads of sum_d max(q_d * low_d, q_d * high_d); ties go to the
     earlier page.  Pages keep the sequence's order; -1 pads a sequence that has fewer."""
-    import torch
-
-    cabi = _cabi()
-    dtype = _element_code(torch, q.dtype)
-    _check_bounds(torch, key_bounds, q.dtype)
-    kv_heads, dim = key_bounds.shape[1], key_bounds.shape[3]
-    q = _check_query(torch, q, kv_heads, dim)
-    _check_take(num_pages)
+    dtype = _element_code(q.dtype)
+    _check_bounds(key_bounds, q.dtype)
     _require(page_size >= TILE_TOKENS and page_size % TILE_TOKENS == 0, "page_size must be a multiple of 16")
-    device = key_bounds.device
-    _require(q.device == device and block_table.device == device and seq_lens.device == device,
-             "q, key bounds, page table and lengths must share one CUDA device")
-    batch = q.shape[0]
-    page_table = torch.empty((batch, kv_heads, num_pages), dtype=torch.int32, device=device)
-    page_lens = torch.empty((batch, kv_heads), dtype=torch.int32, device=device)
-    args = _paged(torch, cabi, batch, kv_heads, dim, page_size, key_bounds.shape[0], dtype, block_table, seq_lens,
-                  per_head=False, q=q, bounds=key_bounds, page_table=page_table, page_lens=page_lens, take=num_pages)
-    with cabi.device_of(key_bounds):
-        scratch = _add_workspace(torch, cabi, args, cabi.INT4_SELECT, device)
-        cabi.check(cabi.library().qf_select_kv_pages(ctypes.byref(args), cabi.stream_pointer(device)))
+    pages, kv_heads, _, dim = key_bounds.shape
+    geometry = (pages, kv_heads, dim, page_size)
+    q = _check_query(q, geometry)
+    _check_take(num_pages)
+    device = key_bounds.get_device()
+    _require(q.get_device() == device, _PAGED_DEVICE)
+    choice = _empty_choice(q.shape[0], kv_heads, num_pages, q.device)
+    cabi = _cabi()
+    args, scratch = _paged(device, q.shape[0], geometry, dtype, block_table, seq_lens, q=q, bounds=key_bounds, choice=choice,
+                           take=num_pages, call=cabi.INT4_SELECT)
+    _enqueue(cabi.library().qf_select_kv_pages, ctypes.byref(args), device=device)
     del scratch
-    return page_table, page_lens
+    return choice
 
 
 def sparse_decode_attention_int4(q, kv4_pool, key_bounds, block_table, seq_lens, *, num_pages, scale=None):
     """select_kv_pages and paged_decode_attention_int4 over its choice in one call: (out, page_table,
     page_lens).  key_bounds must be up to date for every page but a sequence's newest."""
-    import torch
-
-    cabi = _cabi()
-    kv_heads, dim, page_size = _check_pool(torch, kv4_pool)
-    dtype = _element_code(torch, q.dtype)
-    _check_bounds(torch, key_bounds, q.dtype)
-    _require(key_bounds.shape[0] == kv4_pool.shape[0] and key_bounds.shape[1] == kv_heads and key_bounds.shape[3] == dim,
-             "key bounds do not match the pool")
-    q = _check_query(torch, q, kv_heads, dim)
+    geometry = _check_pool(kv4_pool)
+    dtype = _element_code(q.dtype)
+    _check_bounds(key_bounds, q.dtype, geometry)
+    q = _check_query(q, geometry)
     _check_take(num_pages)
-    device = kv4_pool.device
-    _require(q.device == device and key_bounds.device == device and block_table.device == device
-             and seq_lens.device == device, "q, pool, key bounds, page table and lengths must share one CUDA device")
-    batch = q.shape[0]
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    page_table = torch.empty((batch, kv_heads, num_pages), dtype=torch.int32, device=device)
-    page_lens = torch.empty((batch, kv_heads), dtype=torch.int32, device=device)
-    args = _paged(torch, cabi, batch, kv_heads, dim, page_size, kv4_pool.shape[0], dtype, block_table, seq_lens,
-                  per_head=False, q=q, out=out, pool=kv4_pool, bounds=key_bounds, page_table=page_table,
-                  page_lens=page_lens, take=num_pages, scale=dim ** -0.5 if scale is None else scale)
-    with cabi.device_of(kv4_pool):
-        scratch = _add_workspace(torch, cabi, args, cabi.INT4_SPARSE, device)
-        cabi.check(cabi.library().qf_int4_sparse_decode_attention(ctypes.byref(args), cabi.stream_pointer(device)))
+    device = kv4_pool.get_device()
+    _require(q.get_device() == device and key_bounds.get_device() == device, _PAGED_DEVICE)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    choice = _empty_choice(q.shape[0], geometry[1], num_pages, q.device)
+    cabi = _cabi()
+    args, scratch = _paged(device, q.shape[0], geometry, dtype, block_table, seq_lens, q=q, out=out, pool=kv4_pool,
+                           bounds=key_bounds, choice=choice, take=num_pages,
+                           scale=geometry[2] ** -0.5 if scale is None else scale, call=cabi.INT4_SPARSE)
+    _enqueue(cabi.library().qf_int4_sparse_decode_attention, ctypes.byref(args), device=device)
     del scratch
-    return out, page_table, page_lens
+    return out, *choice

@@ -45,7 +45,7 @@ def _write_args(cabi, **changes):
     (dict(k=None), b"must not be null"), (dict(pool=8), b"aligned"), (dict(q_heads=4), b"q and q_out"),
     (dict(positions=16, positions_dtype=3), b"positions"), (dict(positions=16, positions_dtype=2, rope_table=16, table_positions=4), b"positions"),
     (dict(positions=16, base=0.0), b"base"), (dict(positions=16, rope_table=16), b"table is empty"),
-    (dict(slot_mapping=16, slot_dtype=2), b"slot mapping"), (dict(num_pages=-1), b"num_pages"),
+    (dict(slot_mapping=16, slot_dtype=2), b"slot mapping"), (dict(num_pages=-1), b"2^31 slots"), (dict(num_pages=1 << 27), b"2^31 slots"), (dict(rows=(1 << 31) - 1), b"too many rows"),
 ])
 def test_write_refusals(package, changes, message):
     lib = package.cabi.library()
@@ -97,7 +97,7 @@ def test_paged_refusals(package, changes, message):
     args = _paged_args(package.cabi, **changes)
     assert lib.qf_int4_sparse_decode_attention(ctypes.byref(args), None) != 0
     # without a GPU the status word has no address, which is the last of the checks before the workspace's
-    assert message in lib.qf_last_error() or b"status word" in lib.qf_last_error() and "workspace" in str(changes)
+    assert message in lib.qf_last_error() or b"status word" in lib.qf_last_error() and "workspace" in str(changes), lib.qf_last_error()
 
 
 def test_workspace_sizes(package):
