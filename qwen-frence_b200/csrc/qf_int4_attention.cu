@@ -20,6 +20,9 @@
 // their tiles are done.  A row that one warp holds whole is written from its registers; what the
 // warps of a CTA hold of one row is summed at the CTA's end, and rows that span CTAs by a second
 // kernel, in the order of the tiles: the same call gives the same bits.
+#include <algorithm>
+#include <atomic>
+
 #include "qf_int4_paged.cuh"
 
 namespace qf {
@@ -32,11 +35,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D, int NT>
 struct Shape {
-  static constexpr int kWarps = NT == 1 ? 16 : 8;
+  static constexpr int kWarps = NT == 2 ? 8 : D == 128 ? 12 : 16;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kTileBytes = 20 * D;
   static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = 208 * 1024 / kWarps / kStageBytes;  // of a warp's ring: one less in flight
+  static constexpr int kStages = 204 * 1024 / kWarps / kStageBytes;  // of a warp's ring: one less in flight
   static constexpr int kRing = kStages * kStageBytes;
   static constexpr int kHeads = 8 * NT;        // query heads a row has room for
   static constexpr int kStride = D + 4;        // floats between heads of a piece: its float4 stores miss no bank
@@ -46,7 +49,7 @@ struct Shape {
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -59,14 +62,14 @@ __device__ __forceinline__ void mma_t<__half>(float (&c)[4], uint32_t a0, uint32
 template <>
 __device__ __forceinline__ void mma_t<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                                      uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // 8 x 8 transpose of 16-bit elements across the warp.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
@@ -103,12 +106,13 @@ __device__ __forceinline__ int row_tokens_at(const PagedInt4& p, int row) {
 }
 
 // Shared by a CTA's warps: prefix sums of the rows' units, thread by thread (`chunk` rows each),
-// and, where a thread has one row, the rows' lengths.
+// and the lengths of the first rows.
+constexpr int kRowsKept = 2048;
 template <int kWarps>
 struct Shares {
   int prefix[32 * kWarps];
-  int tokens[32 * kWarps];
   int warp[kWarps];
+  int tokens[kRowsKept];
 };
 
 template <int kWarps>
@@ -119,7 +123,7 @@ __device__ __forceinline__ Plan make_plan(const PagedInt4& p, Shares<kWarps>& s,
   for (int r = first; r < first + chunk && r < rows; ++r) {
     const int tokens = row_tokens_at(p, r);
     mine += (tokens + kUnit - 1) / kUnit;
-    s.tokens[threadIdx.x] = tokens;
+    if (r < kRowsKept) s.tokens[r] = tokens;
   }
   int sum = mine;
 #pragma unroll
@@ -154,32 +158,23 @@ __device__ __forceinline__ int2 find_rows(const Shares<kWarps>& s, int first, in
   return make_int2(32 * warp + thread, __shfl_sync(0xffffffffu, start, thread));
 }
 
-// Lengths of 32 rows, a lane each.
-struct Lengths {
-  int base, tokens;
-  const int* shared;  // the lengths of all rows in shared memory, if they are there
-  __device__ __forceinline__ void load(const PagedInt4& p, int row, int lane) {
-    base = row;
-    tokens = row + lane >= p.batch * p.kv_heads ? 0 : shared != nullptr ? shared[row + lane] : row_tokens_at(p, row + lane);
-  }
-  __device__ __forceinline__ int of(const PagedInt4& p, int row, int lane) {
-    if (row - base >= 32) load(p, row, lane);
-    return __shfl_sync(0xffffffffu, tokens, row - base);
-  }
-};
+template <int kWarps>
+__device__ __forceinline__ int tokens_of(const PagedInt4& p, const Shares<kWarps>& s, int row) {
+  return row < kRowsKept ? s.tokens[row] : row_tokens_at(p, row);
+}
 
 // The next 32 units to request: lane i holds the two tiles of unit i, kNoTile for one behind the
 // row's end or in a page outside the pool.
 struct Requests {
-  Lengths lengths;
   int row, unit;  // the next one
   int left;
   uint32_t tile[2];
 
-  __device__ __forceinline__ void refill(const PagedInt4& p, int lane) {
+  template <int kWarps>
+  __device__ __forceinline__ void refill(const PagedInt4& p, const Shares<kWarps>& s, int lane) {
     int filled = 0, mine = -1, mine_row = 0, mine_tokens = 0;
     while (filled < 32 && left > 0 && row < p.batch * p.kv_heads) {
-      const int tokens = lengths.of(p, row, lane);
+      const int tokens = tokens_of(p, s, row);
       const int units = (tokens + kUnit - 1) / kUnit;
       const int n = min(min(32 - filled, units - unit), left);
       if (lane >= filled && lane < filled + n) mine = unit + lane - filled, mine_row = row, mine_tokens = tokens;
@@ -204,23 +199,30 @@ struct Pair;
 template <>
 struct Pair<__half> {
   using type = __half2;
+  static constexpr bool kFine = true;
   static __device__ __forceinline__ __half2 of(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 };
 template <>
 struct Pair<__nv_bfloat16> {
   using type = __nv_bfloat162;
+  static constexpr bool kFine = false;
   static __device__ __forceinline__ __nv_bfloat162 of(uint32_t x) { return *reinterpret_cast<__nv_bfloat162*>(&x); }
 };
 
 template <typename T, int D, int NT>
 struct Row {
   static constexpr int W = D / kInt4Group;
+  // A rounded weight is off by 2^-12 of itself on average, times a code of 7.5 on average.  For fp16
+  // results the codes count from 7.5: sum_t (p c) m = sum_t fl(p c) (m - 7.5) + 7.5 sum_t p c but for the
+  // rounding of fl, now times |m - 7.5|.  bf16 results are rounded coarser than either.
+  static constexpr bool kCentred = Pair<T>::kFine;
   uint32_t q[NT][2 * W][2];   // B fragments of the codes' product, two k-steps a group
   uint32_t qs[NT][2];         // and of the floors' product
   float c[NT][2];             // log2 units per unit of the products, heads 2t and 2t + 1 of an n-tile
   float o[NT][2 * W][4];
   uint64_t z[NT][W / 2][2];   // this lane's tokens' p * floor: pairs of groups, head 2t or 2t + 1
   float l[NT][2];             // and p
+  float h[NT][4];             // fp16: 7.5 times the rounded weights of group g, heads 2t and 2t + 1 (half of the lanes')
   float off[NT][2];           // largest score so far (of the last raise) + e - 10
   int e;
 
@@ -302,7 +304,7 @@ struct Row {
       c[i][1] = __shfl_sync(0xffffffffu, scale, 8 * t + 4);
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        l[i][y] = 0.f, off[i][y] = -INFINITY;
+        l[i][y] = 0.f, off[i][y] = -INFINITY, h[i][y] = h[i][2 + y] = 0.f;
 #pragma unroll
         for (int w = 0; w < W / 2; ++w) z[i][w][y] = 0u;
       }
@@ -364,6 +366,7 @@ struct Row {
         const float keep = fast_exp2(off[i][y] - raised);
         off[i][y] = raised;
         l[i][y] *= keep;
+        h[i][y] *= keep;
 #pragma unroll
         for (int w = 0; w < W / 2; ++w) z[i][w][y] = mul32x2(z[i][w][y], pair32(keep, keep));
 #pragma unroll
@@ -478,7 +481,9 @@ struct Row {
         for (int w = 0; w < W / 2; ++w) {
           const float2 s0 = unpack2<T>(vc[2 * k][w]), s1 = unpack2<T>(vc[2 * k + 1][w]);
           const float2 f0 = unpack2<T>(ve[2 * k][w]), f1 = unpack2<T>(ve[2 * k + 1][w]);
-          const uint64_t c0 = pair32(s0.x, s0.y), c1 = pair32(s1.x, s1.y), e0 = pair32(f0.x, f0.y), e1 = pair32(f1.x, f1.y);
+          const uint64_t c0 = pair32(s0.x, s0.y), c1 = pair32(s1.x, s1.y);
+          uint64_t e0 = pair32(f0.x, f0.y), e1 = pair32(f1.x, f1.y);
+          if constexpr (kCentred) e0 = fma32x2(c0, pair32(7.5f, 7.5f), e0), e1 = fma32x2(c1, pair32(7.5f, 7.5f), e1);
           z[i][w][0] = fma32x2(twice[0], e0, fma32x2(twice[2], e1, z[i][w][0]));
           z[i][w][1] = fma32x2(twice[1], e0, fma32x2(twice[3], e1, z[i][w][1]));
           const float2 p0 = unpair32(mul32x2(twice[0], c0)), p1 = unpair32(mul32x2(twice[1], c0));
@@ -494,6 +499,10 @@ struct Row {
         const uint32_t u0 = v0[w] >> 8, u1 = v1[w] >> 8;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
+          if constexpr (kCentred) {  // 7.5 in row w of an A that is zero elsewhere: one sum for all groups
+            const uint32_t ones = g == w ? 0x47804780u : 0u;
+            mma_f16(h[i], ones, 0u, ones, 0u, pb[i][w][0], pb[i][w][1]);
+          }
           mma_f16(o[i][2 * w], v0[w] & 0x000f000fu, v0[w] & 0x00f000f0u, v1[w] & 0x000f000fu, v1[w] & 0x00f000f0u, pb[i][w][0], pb[i][w][1]);
           mma_f16(o[i][2 * w + 1], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, pb[i][w][0], pb[i][w][1]);
         }
@@ -502,7 +511,8 @@ struct Row {
   }
 
   // Sum the lanes' tokens: every lane then holds l and o (heads 2t, 2t + 1, channels 32w + 4g + 0..3).
-  __device__ __forceinline__ void finish() {
+  __device__ __forceinline__ void finish(int lane) {
+    const int t = lane & 3;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
 #pragma unroll
@@ -515,6 +525,7 @@ struct Row {
           float sum = w % 2 ? both.y : both.x;
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+          if constexpr (kCentred) sum -= __shfl_sync(0xffffffffu, h[i][y], 4 * w + t);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             o[i][2 * w + k][y] = fmaf(o[i][2 * w + k][y], 16777216.f, sum);
@@ -622,18 +633,18 @@ __device__ __forceinline__ float warp_sum(float x) {
 
 // Scratch: two pieces a CTA for the second kernel (the row it shares with the CTAs before it, the
 // row it starts and shares with those behind), one a warp for the row a warp shares with the warps
-// before it, and the first and last CTA of every row.
+// before it, and for every CTA the row that it starts and shares (-1: none) and the last CTA of it.
 struct Scratch {
   float* cta_pieces;
   float* warp_pieces;
-  int2* spans;
+  int2* shared_rows;
 };
 template <int D, int NT>
 __host__ __device__ Scratch carve(void* workspace, int ctas) {
   Scratch s;
   s.cta_pieces = static_cast<float*>(workspace);
   s.warp_pieces = s.cta_pieces + static_cast<int64_t>(2 * ctas) * Shape<D, NT>::kPiece;
-  s.spans = reinterpret_cast<int2*>(s.warp_pieces + static_cast<int64_t>(Shape<D, NT>::kWarps * ctas) * Shape<D, NT>::kPiece);
+  s.shared_rows = reinterpret_cast<int2*>(s.warp_pieces + static_cast<int64_t>(Shape<D, NT>::kWarps * ctas) * Shape<D, NT>::kPiece);
   return s;
 }
 
@@ -645,6 +656,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
   __shared__ Shares<kWarps> s_shares;
   __shared__ int s_row[2 * kWarps];    // rows of the pieces left to merge, warp by warp (first, last), -1: none
   __shared__ int s_flags[2 * kWarps];  // kRowStart / kRowEnd of those pieces
+  __shared__ int2 s_shared_row;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ctas = gridDim.x, cta = blockIdx.x;
@@ -652,6 +664,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
   const Scratch scratch = carve<D, NT>(p.workspace, ctas);
   uint8_t* ring = s_ring + warp * S::kRing;
   if (threadIdx.x < 2 * kWarps) s_row[threadIdx.x] = -1;
+  if (threadIdx.x == 0) s_shared_row = make_int2(-1, -1);
   release_dependents();
   if (!p.early) dependency_wait();
   const Plan plan = make_plan(p, s_shares, chunk, ctas);
@@ -668,11 +681,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
       const int2 found = find_rows(s_shares, first, lane);
       ahead.row = found.x * chunk;
       int before = first - found.y;
-      ahead.lengths.shared = chunk == 1 ? s_shares.tokens : nullptr;
-      ahead.lengths.load(p, ahead.row, lane);
       const int rows = p.batch * p.kv_heads;
       while (ahead.row < rows) {
-        const int in_row = (ahead.lengths.of(p, ahead.row, lane) + kUnit - 1) / kUnit;
+        const int in_row = (tokens_of(p, s_shares, ahead.row) + kUnit - 1) / kUnit;
         if (before < in_row) break;
         before -= in_row;
         ++ahead.row;
@@ -681,9 +692,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
       ahead.left = units;
     }
   }
-  Lengths lengths = ahead.lengths;
   int id = ahead.row, in_row = ahead.unit;  // of the unit at hand
-  if (units > 0) ahead.refill(p, lane);
+  if (units > 0) ahead.refill(p, s_shares, lane);
   if (p.early) dependency_wait();
 
   if (units > 0) {
@@ -698,7 +708,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
     // One group of copies a call, an empty one behind the last unit.
     auto request = [&]() {
       if (wanted < units) {
-        if ((wanted & 31) == 0 && wanted > 0) ahead.refill(p, lane);
+        if ((wanted & 31) == 0 && wanted > 0) ahead.refill(p, s_shares, lane);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const uint32_t tile = __shfl_sync(0xffffffffu, ahead.tile[k], wanted & 31);
@@ -724,7 +734,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
     while (done < units) {
       int tokens = 0;
       while (id < p.batch * p.kv_heads) {
-        tokens = lengths.of(p, id, lane);
+        tokens = tokens_of(p, s_shares, id);
         if (in_row * kUnit < tokens) break;
         ++id, in_row = 0;
       }
@@ -733,8 +743,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
       if (done > 0) row.load(p, id, group, lane, queries);
       row.start(p, queries, lane);
       const bool starts = in_row == 0, ends = in_row + n >= in_all;
-      // the CTAs that hold the row: this one and those its last unit reaches
-      if (starts && lane == 0) scratch.spans[id] = make_int2(cta, (first + done + in_all - 1) / plan.share);
+      if (starts && lane == 0) {
+        const int beyond = first + done + in_all - cta_first;  // units of the row's end from this CTA's first on
+        if (beyond > cta_units) s_shared_row = make_int2(id, cta + (beyond - 1) / plan.share);
+      }
       int left = tokens - in_row * kUnit;
       for (int k = 0; k < n; ++k, left -= kUnit) {
         copies_wait<S::kStages - 2>();
@@ -744,7 +756,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
         at = at + S::kStageBytes == ring + S::kRing ? ring : at + S::kStageBytes;
       }
       done += n;
-      row.finish();
+      row.finish(lane);
       if (starts && ends) {
         row.write_out(p, id, group, lane);
       } else {
@@ -760,6 +772,17 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
     }
   }
   __syncthreads();
+
+  if (threadIdx.x == 0) scratch.shared_rows[cta] = s_shared_row;
+  // rows without tokens
+  for (int r = cta; r < p.batch * p.kv_heads; r += ctas) {
+    if (tokens_of(p, s_shares, r) != 0) continue;
+    const int2 at = row_place(p, r);
+    for (int i = threadIdx.x; i < group * (D / 8); i += S::kThreads) {
+      const int head = at.y * group + i / (D / 8), d = i % (D / 8) * 8;
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at.x * p.o_sb + head * p.o_sh + d) = make_uint4(0, 0, 0, 0);
+    }
+  }
 
   // Rows that several warps, or several CTAs, hold: a warp takes a head, a lane the offset and the
   // sum of one piece.
@@ -777,8 +800,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
     rest &= ~chain;
     const bool starts = (__shfl_sync(0xffffffffu, my_flags, i) & kRowStart) != 0;
     const bool ends = (__shfl_sync(0xffffffffu, my_flags, 31 - __clz(chain)) & kRowEnd) != 0;
-    int head = (warp - item) & (kWarps - 1);
-    item += group;
+    int head = warp - item + (warp < item ? kWarps : 0);
+    item = (item + group) % kWarps;
     for (; head < group; head += kWarps) {
       float2 ml = make_float2(-INFINITY, 0.f);
       if (my_row == id) ml = *reinterpret_cast<const float2*>(piece_of(lane) + S::kHeads * S::kStride + 2 * head);
@@ -811,92 +834,80 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
   }
 }
 
-// Rows that span CTAs, and zeros for rows without tokens: one CTA of four warps a (row, head),
-// the pieces dealt out to the warps in turn.
+// Rows that span CTAs: one CTA a CTA of the first kernel, for the row that starts there and goes on,
+// `each` warps a query head, the pieces dealt out to those in turn.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128) int4_combine_kernel(const PagedInt4 p, int ctas, Divisor by_group) {
+__global__ void __launch_bounds__(1024) int4_combine_kernel(const PagedInt4 p, int ctas, int each) {
   using S = Shape<D, NT>;
   constexpr int C = Merge<D>::C;
-  __shared__ float s_o[4][D];
-  __shared__ float s_top[4], s_sum[4];
+  __shared__ float s_o[32][D];
+  __shared__ float s_top[32], s_sum[32];
   release_dependents();
-  if (!p.early) dependency_wait();
-  const int group = by_group.d;
-  const int row = quotient(blockIdx.x, by_group), head = blockIdx.x - row * group;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  dependency_wait();
   const Scratch scratch = carve<D, NT>(p.workspace, ctas);
-  const int tokens = row_tokens_at(p, row);
-  if (p.early) dependency_wait();
-  const int2 span = scratch.spans[row];  // unwritten, and not used, for a row without tokens
-  if (tokens == 0) {
-    const int2 at = row_place(p, row);
-    T* dst = static_cast<T*>(p.out) + at.x * p.o_sb + (static_cast<int64_t>(at.y) * group + head) * p.o_sh;
-    for (int d = threadIdx.x; d < D; d += 128) dst[d] = from_float<T>(0.f);
-    return;
-  }
-  if (span.x == span.y) return;
-  auto piece_of = [&](int c) { return scratch.cta_pieces + static_cast<int64_t>(2 * c + (c == span.x ? 1 : 0)) * S::kPiece; };
-  // offset and sum of every piece, a lane each, 128 at a time; every warp sees all of them
+  const int2 shared = scratch.shared_rows[blockIdx.x];
+  const int row = shared.x, from = blockIdx.x, to = shared.y;
+  if (row < 0) return;
+  const int group = p.q_heads / p.kv_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int head = warp / each, part = warp % each;
+  auto piece_of = [&](int c) { return scratch.cta_pieces + static_cast<int64_t>(2 * c + (c == from ? 1 : 0)) * S::kPiece; };
   float top = -INFINITY, sum = 0.f;
   Merge<D> merge;
   merge.clear();
-  for (int first = span.x; first <= span.y; first += 128) {
+  // offset and sum of 32 pieces of this warp at a time, a lane each
+  for (int first = from + part; first <= to; first += 32 * each) {
+    const int n = min(32, (to - first) / each + 1);
     float2 ml = make_float2(-INFINITY, 0.f);
-    const int mine = first + 4 * lane + warp;  // a warp's pieces are every fourth
-    if (mine <= span.y) ml = *reinterpret_cast<const float2*>(piece_of(mine) + S::kHeads * S::kStride + 2 * head);
+    if (lane < n) ml = *reinterpret_cast<const float2*>(piece_of(first + each * lane) + S::kHeads * S::kStride + 2 * head);
+    float x[4][C];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) Merge<D>::load(piece_of(first + each * min(y, n - 1)) + head * S::kStride + lane * C, x[y]);
     const float now = fmaxf(top, warp_max(ml.x));
     const float keep = sum == 0.f ? 0.f : fast_exp2(top - now);
-    const float weight = mine <= span.y ? fast_exp2(ml.x - now) : 0.f;
+    const float weight = lane < n ? fast_exp2(ml.x - now) : 0.f;
     top = now;
     sum = sum * keep + warp_sum(ml.y * weight);
 #pragma unroll
     for (int c = 0; c < C; ++c) merge.o[c] *= keep;
-    const int n = min(32, (span.y - first - warp + 4) / 4);  // pieces of this warp in this turn
     for (int k = 0; k < n; k += 4) {
-      float x[4][C];
+      float next[4][C];
 #pragma unroll
-      for (int y = 0; y < 4; ++y) Merge<D>::load(piece_of(first + 4 * min(k + y, n - 1) + warp) + head * S::kStride + lane * C, x[y]);
+      for (int y = 0; y < 4; ++y) {
+        if (k + 4 < n) Merge<D>::load(piece_of(first + each * min(k + 4 + y, n - 1)) + head * S::kStride + lane * C, next[y]);
+      }
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const float scale = __shfl_sync(0xffffffffu, weight, (k + y) & 31);
-        merge.add(x[y], k + y < n ? scale : 0.f);
+        if (k + y < n) merge.add(x[y], scale);
+#pragma unroll
+        for (int c = 0; c < C; ++c) x[y][c] = next[y][c];
       }
     }
   }
-#pragma unroll
-  for (int c = 0; c < C; ++c) s_o[warp][lane * C + c] = merge.o[c];
+  Merge<D>::store(&s_o[warp][lane * C], merge.o);
   if (lane == 0) s_top[warp] = top, s_sum[warp] = sum;
   __syncthreads();
-  if (warp != 0) return;
-  const int warps = min(4, span.y - span.x + 1);
-  float all = s_top[0];
-  for (int w = 1; w < warps; ++w) all = fmaxf(all, s_top[w]);
+  if (part != 0) return;
+  const int parts = min(each, to - from + 1);
+  float all = top;
+  for (int w = 1; w < parts; ++w) all = fmaxf(all, s_top[warp + w]);
   sum = 0.f;
   merge.clear();
-  for (int w = 0; w < warps; ++w) {
-    const float weight = fast_exp2(s_top[w] - all);
+  for (int w = 0; w < parts; ++w) {
+    const float weight = fast_exp2(s_top[warp + w] - all);
     float x[C];
-    Merge<D>::load(&s_o[w][lane * C], x);
+    Merge<D>::load(&s_o[warp + w][lane * C], x);
     merge.add(x, weight);
-    sum = fmaf(s_sum[w], weight, sum);
+    sum = fmaf(s_sum[warp + w], weight, sum);
   }
   merge.template write_out<T>(p, row, group, head, lane, sum);
 }
 
-int sm_count() {
-  int device = 0, count = 0;
-  if (cudaGetDevice(&device) != cudaSuccess ||
-      cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return 148;
-  }
-  return count;
-}
-
 template <int D, int NT>
-int64_t scratch_bytes(int64_t rows, int ctas) {
+int64_t scratch_bytes(int ctas) {
   const int64_t pieces = static_cast<int64_t>(2 + Shape<D, NT>::kWarps) * ctas * Shape<D, NT>::kPiece * 4;
-  return (pieces + rows * 8 + 15) / 16 * 16;
+  return (pieces + 8 * ctas + 15) / 16 * 16;
 }
 
 template <typename T, int D, int NT>
@@ -904,10 +915,9 @@ int launch(const PagedInt4& p, cudaStream_t stream) {
   using S = Shape<D, NT>;
   const int64_t rows = static_cast<int64_t>(p.batch) * p.kv_heads;
   const int ctas = sm_count();
-  const int64_t need = scratch_bytes<D, NT>(rows, ctas);
+  const int64_t need = scratch_bytes<D, NT>(ctas);
   QF_REQUIRE(p.workspace != nullptr && p.workspace_bytes >= need, "the workspace holds %lld bytes, %lld are needed",
              static_cast<long long>(p.workspace_bytes), static_cast<long long>(need));
-  QF_REQUIRE(rows * (p.q_heads / p.kv_heads) < (1LL << 31), "too many rows");
   static thread_local int ready = -1;  // device whose kernel attribute this thread has set
   int device = 0;
   QF_CUDA(cudaGetDevice(&device));
@@ -917,8 +927,13 @@ int launch(const PagedInt4& p, cudaStream_t stream) {
   }
   const int chunk = static_cast<int>((rows + S::kThreads - 1) / S::kThreads);
   QF_CUDA(launch_chained(int4_attention_kernel<T, D, NT>, dim3(ctas), dim3(S::kThreads), static_cast<size_t>(S::kSmem), stream, p, chunk));
-  QF_CUDA(launch_chained(int4_combine_kernel<T, D, NT>, dim3(static_cast<unsigned>(rows * (p.q_heads / p.kv_heads))), dim3(128),
-                         static_cast<size_t>(0), stream, p, ctas, make_divisor(p.q_heads / p.kv_heads)));
+  // warps a head in the second kernel, four pieces each or more: a row is on all CTAs' share of the
+  // rows at most, and on as many CTAs as its table has room for
+  const int group = p.q_heads / p.kv_heads;
+  const int64_t row_units = (p.table_width * p.page_size + kUnit - 1) / kUnit;
+  const int64_t row_ctas = std::min<int64_t>(ctas / rows, row_units / S::kWarps) / 4;
+  const int each = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(row_ctas, group <= 8 ? 4 : 2)));
+  QF_CUDA(launch_chained(int4_combine_kernel<T, D, NT>, dim3(ctas), dim3(32 * group * each), static_cast<size_t>(0), stream, p, ctas, each));
   QF_CUDA(cudaGetLastError());
   return QF_OK;
 }
@@ -932,14 +947,27 @@ int launch_for(const PagedInt4& p, int head_dim, cudaStream_t stream) {
 
 }  // namespace
 
-int64_t int4_attention_bytes(const PagedInt4& p, int head_dim) {
-  const int64_t rows = static_cast<int64_t>(p.batch) * p.kv_heads;
-  const bool two = p.q_heads / p.kv_heads > 8;
-  const int sms = sm_count();
-  if (head_dim == 128) {
-    return two ? scratch_bytes<128, 2>(rows, sms) : scratch_bytes<128, 1>(rows, sms);
+int sm_count() {
+  static std::atomic<int> counts[64];  // 0: not asked yet; the answer never changes
+  int device = 0, count = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 148;
   }
-  return two ? scratch_bytes<64, 2>(rows, sms) : scratch_bytes<64, 1>(rows, sms);
+  if (device < 64 && (count = counts[device].load(std::memory_order_relaxed)) != 0) return count;
+  if (cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 148;
+  }
+  if (device < 64) counts[device].store(count, std::memory_order_relaxed);
+  return count;
+}
+
+int64_t int4_attention_bytes(const PagedInt4& p, int head_dim) {
+  const bool two = p.q_heads / p.kv_heads > 8;
+  const int ctas = sm_count();
+  if (head_dim == 128) return two ? scratch_bytes<128, 2>(ctas) : scratch_bytes<128, 1>(ctas);
+  return two ? scratch_bytes<64, 2>(ctas) : scratch_bytes<64, 1>(ctas);
 }
 
 int launch_int4_attention(const PagedInt4& p, int head_dim, int dtype, cudaStream_t stream) {

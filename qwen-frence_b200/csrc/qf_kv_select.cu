@@ -5,6 +5,8 @@
 // (sequence, KV head) takes its newest page and the take - 1 others that score highest, ties
 // to the lower page.  The products are exact in fp32 and are added pairwise, neighbours first,
 // whatever the kernel's layout: the same inputs choose the same pages everywhere.
+#include <algorithm>
+
 #include "qf_int4_paged.cuh"
 
 namespace qf {
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(128) page_score_kernel(const PagedInt4 p, uint
   constexpr int kLanes = D / 8, kPages = 32 / kLanes, kMaxGroup = 16, kCtaPages = 4 * 2 * kPages;
   __shared__ __align__(16) float4 s_q[kMaxGroup][4][kLanes];  // two channels of a lane: neighbouring lanes, neighbouring banks
   release_dependents();
-  dependency_wait();
+  if (!p.early) dependency_wait();
   const int row = blockIdx.y;
   const int2 at = row_place(p, row);
   const int b = at.x, h = at.y;
@@ -200,7 +202,38 @@ __global__ void __launch_bounds__(128) page_score_kernel(const PagedInt4 p, uint
   const int group = p.q_heads / p.kv_heads;
   const int tokens = static_cast<int>(row_tokens(p, b, 0));
   const int count = quotient(tokens + p.page_size - 1, p.by_page);
-  if (count <= p.take || static_cast<int>(blockIdx.x) * kCtaPages >= count - 1) return;  // every page is taken, or none is left
+  const bool idle = count <= p.take || static_cast<int>(blockIdx.x) * kCtaPages >= count - 1;  // every page is taken, or none is left
+  const int step = gridDim.x * kCtaPages;
+  int first = blockIdx.x * kCtaPages + threadIdx.x / 32 * 2 * kPages;
+  int64_t page[2];  // of this turn
+  auto find = [&](int from) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int n = from + k * kPages + lane / kLanes;
+      page[k] = n < count - 1 ? page_id(p, b, 0, n) : -1;
+      if (n < count - 1 && (page[k] < 0 || page[k] >= p.num_pages)) {
+        page[k] = -1;
+        if (l == 0) atomicMax(p.status, kStatusBadPageId);
+      }
+    }
+  };
+  if (!idle) find(first);
+  if (p.early) dependency_wait();
+  if (idle) return;
+  uint4 lo[2], hi[2];
+  bool ok[2];
+  auto fetch = [&]() {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      ok[k] = page[k] >= 0;
+      lo[k] = hi[k] = make_uint4(0, 0, 0, 0);
+      if (ok[k]) {
+        const T* src = static_cast<const T*>(p.bounds) + (page[k] * p.kv_heads + h) * 2 * D + 8 * l;
+        lo[k] = *reinterpret_cast<const uint4*>(src), hi[k] = *reinterpret_cast<const uint4*>(src + D);
+      }
+    }
+  };
+  fetch();
   for (int i = threadIdx.x; i < group * (D / 8); i += 128) {
     const int g = i / (D / 8), d = i % (D / 8) * 8;
     const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_sb + static_cast<int64_t>(h * group + g) * p.q_sh + d);
@@ -211,27 +244,18 @@ __global__ void __launch_bounds__(128) page_score_kernel(const PagedInt4 p, uint
     }
   }
   __syncthreads();
-  for (int first = blockIdx.x * kCtaPages + threadIdx.x / 32 * 2 * kPages; first < count - 1; first += gridDim.x * kCtaPages) {
-    uint4 lo[2], hi[2];
-    bool ok[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int n = first + k * kPages + lane / kLanes;
-      const int64_t page = n < count - 1 ? page_id(p, b, 0, n) : -1;
-      ok[k] = page >= 0 && page < p.num_pages;
-      if (!ok[k] && n < count - 1 && l == 0) atomicMax(p.status, kStatusBadPageId);
-      lo[k] = hi[k] = make_uint4(0, 0, 0, 0);
-      if (ok[k]) {
-        const T* src = static_cast<const T*>(p.bounds) + (page * p.kv_heads + h) * 2 * D + 8 * l;
-        lo[k] = *reinterpret_cast<const uint4*>(src), hi[k] = *reinterpret_cast<const uint4*>(src + D);
-      }
-    }
+  for (; first < count - 1; first += step) {
     uint64_t low[8], high[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 a = unpack2<T>((&lo[0].x)[j]), c = unpack2<T>((&lo[1].x)[j]), y = unpack2<T>((&hi[0].x)[j]), z = unpack2<T>((&hi[1].x)[j]);
       low[2 * j] = pair32(a.x, c.x), low[2 * j + 1] = pair32(a.y, c.y);
       high[2 * j] = pair32(y.x, z.x), high[2 * j + 1] = pair32(y.y, z.y);
+    }
+    const bool now[2] = {ok[0], ok[1]};
+    if (first + step < count - 1) {  // the next turn's bounds come in meanwhile
+      find(first + step);
+      fetch();
     }
     float best[2] = {-INFINITY, -INFINITY};
     for (int g = 0; g < group; ++g) {
@@ -254,7 +278,7 @@ __global__ void __launch_bounds__(128) page_score_kernel(const PagedInt4 p, uint
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int n = first + k * kPages + lane / kLanes;
-      if (l == 0 && n < count - 1) keys[static_cast<int64_t>(row) * p.table_width + n] = ok[k] ? score_key(best[k]) : 0u;
+      if (l == 0 && n < count - 1) keys[static_cast<int64_t>(row) * p.table_width + n] = now[k] ? score_key(best[k]) : 0u;
     }
   }
 }
@@ -386,9 +410,11 @@ int launch_select(const PagedInt4& p, int head_dim, int dtype, cudaStream_t stre
   const int rows = p.batch * p.kv_heads;
   QF_REQUIRE(rows <= 65535, "at most 65535 (sequence, KV head) rows choose pages in one call");
   uint32_t* keys = static_cast<uint32_t*>(p.workspace);
-  const int64_t pages = head_dim == 128 ? 16 : 32;  // of a CTA at a time
-  const int64_t blocks = (p.table_width + pages - 1) / pages;
-  const dim3 grid(static_cast<unsigned>(blocks < 1 ? 1 : blocks > 2048 ? 2048 : blocks), rows);
+  // A CTA takes 16 pages (D 128) or 32 at a time: all of them at once while that is one wave of
+  // about 900 CTAs, in turns beyond it.
+  const int64_t pages = head_dim == 128 ? 16 : 32;
+  const int64_t blocks = (p.table_width + pages - 1) / pages, most = std::max<int64_t>(1, 900 / rows);
+  const dim3 grid(static_cast<unsigned>(std::max<int64_t>(1, std::min(blocks, most))), rows);
   cudaError_t err = cudaSuccess;
   if (dtype == QF_DTYPE_F16) {
     err = head_dim == 128 ? launch_chained(page_score_kernel<__half, 128>, grid, dim3(128), 0, stream, p, keys)

@@ -95,9 +95,9 @@ def _index_code(tensor, what):
     return code
 
 
-def _enqueue(function, *arguments, device):
+def _enqueue(function, arguments, device):
     """One library call on the current stream of CUDA device number `device`, which is current meanwhile."""
-    cabi = _cabi()
+    cabi = _cabi_module
     if torch.cuda.current_device() == device:
         status = function(*arguments, cabi.raw_stream(device))
     else:
@@ -160,7 +160,7 @@ def _write(pool, geometry, pointers, strides, like, positions, slot_mapping, *, 
     args = cabi.Int4WriteArgs(
         *pointers, *strides, position_at, position_stride, slot_at, slot_stride, table_at, pool.data_ptr(), pages, valid_at,
         rows, q_heads, kv_heads, dim, page_size, dtype, position_code, slot_code, table_positions, base)
-    _enqueue(cabi.library().qf_int4_rope_kv_write, ctypes.byref(args), device=device)
+    _enqueue(cabi.library().qf_int4_rope_kv_write, (ctypes.byref(args),), device)
 
 
 def packed_qkv_rope_cache_int4(
@@ -260,8 +260,9 @@ def _read(kv4_pool, slots, rows, dtype):
     code = _element_code(dtype)
     both = torch.empty((2, rows, kv_heads, dim), dtype=dtype, device=kv4_pool.device)
     at = both.data_ptr()
-    _enqueue(_cabi().library().qf_int4_read_rows, kv4_pool.data_ptr(), pages, page_size, kv_heads, dim, code, *slots, rows,
-             at, at + 2 * rows * kv_heads * dim, device=kv4_pool.get_device())
+    _enqueue(_cabi().library().qf_int4_read_rows,
+             (kv4_pool.data_ptr(), pages, page_size, kv_heads, dim, code, *slots, rows, at, at + 2 * rows * kv_heads * dim),
+             kv4_pool.get_device())
     return both.unbind(0)
 
 
@@ -288,58 +289,66 @@ _workspace_sizes = {}
 _PAGED_DEVICE = "queries, pool, key bounds, page table and lengths must share one CUDA device"
 
 
-def _paged(device, batch, geometry, dtype, block_table, seq_lens, *, q=None, out=None, pool=None, bounds=None, choice=None,
-           new_tokens=0, take=0, scale=0.0, call=None):
-    """Check table and lengths, fill qf_paged_int4_args and add the scratch of `call`: a torch
-    allocation, so it is the stream's, and a captured graph's own.  Returns (args, scratch)."""
+def _scratch(args, call, device, like):
+    """Scratch of one call: a torch allocation, so it is the stream's, and a captured graph's own."""
+    key = (call, device, args.batch, args.q_heads, args.kv_heads, args.head_dim, args.page_size, args.table_width, args.take)
+    need = _workspace_sizes.get(key)
+    if need is None:
+        cabi, size = _cabi(), ctypes.c_int64()
+        with torch.cuda.device(device):
+            cabi.check(cabi.library().qf_paged_int4_workspace(ctypes.byref(args), call, ctypes.byref(size)))
+        if len(_workspace_sizes) >= 4096:
+            _workspace_sizes.clear()
+        need = _workspace_sizes[key] = size.value
+    scratch = torch.empty(need, dtype=torch.uint8, device=like.device)
+    args.workspace = scratch.data_ptr()
+    args.workspace_bytes = need
+    return scratch
+
+
+def _paged(device, batch, geometry, dtype, block_table, seq_lens, per_head, q, out, pool, bounds, choice, new_tokens, take, scale):
+    """Check table and lengths and fill qf_paged_int4_args (no scratch yet)."""
     pages, kv_heads, dim, page_size = geometry
-    cabi = _cabi()
-    t_shape, l_shape = block_table.shape, seq_lens.shape
-    if len(t_shape) == 3 and call == cabi.INT4_ATTENTION:
-        _require(t_shape[:2] == (batch, kv_heads) and l_shape == (batch, kv_heads),
-                 "a table and lengths per KV head have shapes [batch, kv_heads, pages] and [batch, kv_heads]")
-        t_strides, l_strides = block_table.stride(), seq_lens.stride()
+    t_shape = block_table.shape
+    if per_head and len(t_shape) == 3:
+        if t_shape[0] != batch or t_shape[1] != kv_heads or seq_lens.shape != (batch, kv_heads):
+            raise ValueError("a table and lengths per KV head have shapes [batch, kv_heads, pages] and [batch, kv_heads]")
+        t_sb, t_sh, t_sp = block_table.stride()
+        l_sb, l_sh = seq_lens.stride()
     else:
-        _require(len(t_shape) == 2 and t_shape[0] == batch and l_shape == (batch,), "batch dimensions must match")
-        t_strides, l_strides = (block_table.stride(0), 0, block_table.stride(1)), (seq_lens.stride(0), 0)
-    _require(block_table.get_device() == device and seq_lens.get_device() == device, _PAGED_DEVICE)
+        if len(t_shape) != 2 or t_shape[0] != batch or seq_lens.shape != (batch,):
+            raise ValueError("batch dimensions must match")
+        t_sb, t_sp = block_table.stride()
+        l_sb, = seq_lens.stride()
+        t_sh = l_sh = 0
+    if block_table.get_device() != device or seq_lens.get_device() != device:
+        raise ValueError(_PAGED_DEVICE)
     q_at = o_at = pages_at = held_at = None
-    q_heads = q_sb = q_sh = o_sb = o_sh = 0
+    q_heads = q_sb = q_sh = o_sb = 0
     if q is not None:
         q_at, q_heads = q.data_ptr(), q.shape[1]
         q_sb, q_sh, _ = q.stride()
     if out is not None:
-        o_at, o_sb, o_sh = out.data_ptr(), q_heads * dim, dim
+        o_at, o_sb = out.data_ptr(), q_heads * dim
     if choice is not None:
         pages_at, held_at = choice[0].data_ptr(), choice[1].data_ptr()
-    args = cabi.PagedInt4Args(
+    return _cabi().PagedInt4Args(
         q_at, o_at, None if pool is None else pool.data_ptr(), None if bounds is None else bounds.data_ptr(),
-        block_table.data_ptr(), seq_lens.data_ptr(), None, pages_at, held_at, q_sb, q_sh, o_sb, o_sh, *t_strides, *l_strides,
+        block_table.data_ptr(), seq_lens.data_ptr(), None, pages_at, held_at, q_sb, q_sh, o_sb, dim, t_sb, t_sh, t_sp, l_sb, l_sh,
         pages, t_shape[-1], 0, batch, q_heads, kv_heads, dim, page_size, dtype, _index_code(block_table, "page table"),
         _index_code(seq_lens, "lengths"), new_tokens, take, scale)
-    scratch = None
-    if call is not None:
-        key = (call, device, batch, q_heads, kv_heads, dim, page_size, t_shape[-1], take)
-        need = _workspace_sizes.get(key)
-        if need is None:
-            size = ctypes.c_int64()
-            with torch.cuda.device(device):
-                cabi.check(cabi.library().qf_paged_int4_workspace(ctypes.byref(args), call, ctypes.byref(size)))
-            if len(_workspace_sizes) >= 4096:
-                _workspace_sizes.clear()
-            need = _workspace_sizes[key] = size.value
-        scratch = torch.empty(need, dtype=torch.uint8, device=block_table.device)
-        args.workspace, args.workspace_bytes = scratch.data_ptr(), need
-    return args, scratch
 
 
 def _check_query(q, geometry):
     """q as the kernels take it: unit inner stride, rows on 16-byte boundaries."""
     _, kv_heads, dim, _ = geometry
     shape = q.shape
-    _require(len(shape) == 3 and shape[1] >= 1 and shape[2] == dim, "q must have shape [batch, query_heads, head_dim]")
-    _require(shape[1] % kv_heads == 0, "query heads must be divisible by KV heads")
-    _require(shape[1] // kv_heads <= MAX_GROUP, "at most 16 query heads share a KV head")
+    if len(shape) != 3 or shape[1] < 1 or shape[2] != dim:
+        raise ValueError("q must have shape [batch, query_heads, head_dim]")
+    if shape[1] % kv_heads:
+        raise ValueError("query heads must be divisible by KV heads")
+    if shape[1] > MAX_GROUP * kv_heads:
+        raise ValueError("at most 16 query heads share a KV head")
     row, head, inner = q.stride()
     if inner != 1 or row % 8 or head % 8 or q.data_ptr() % 16:
         q = q.contiguous()
@@ -359,12 +368,14 @@ def paged_decode_attention_int4(q, kv4_pool, block_table, seq_lens, *, scale=Non
     dtype = _element_code(q.dtype)
     q = _check_query(q, geometry)
     device = kv4_pool.get_device()
-    _require(q.get_device() == device, _PAGED_DEVICE)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if q.get_device() != device:
+        raise ValueError(_PAGED_DEVICE)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    args = _paged(device, q.shape[0], geometry, dtype, block_table, seq_lens, True, q, out, kv4_pool, None, None, 0, 0,
+                  geometry[2] ** -0.5 if scale is None else scale)
     cabi = _cabi()
-    args, scratch = _paged(device, q.shape[0], geometry, dtype, block_table, seq_lens, q=q, out=out, pool=kv4_pool,
-                           scale=geometry[2] ** -0.5 if scale is None else scale, call=cabi.INT4_ATTENTION)
-    _enqueue(cabi.library().qf_int4_decode_attention, ctypes.byref(args), device=device)
+    scratch = _scratch(args, cabi.INT4_ATTENTION, device, q)
+    _enqueue(cabi.library().qf_int4_decode_attention, (ctypes.byref(args),), device)
     del scratch
     return out
 
@@ -372,11 +383,13 @@ def paged_decode_attention_int4(q, kv4_pool, block_table, seq_lens, *, scale=Non
 def _check_bounds(bounds, dtype, geometry=None):
     """Key bounds of a pool's geometry (default: any)."""
     shape = bounds.shape
-    _require(len(shape) == 4 and shape[2] == 2 and shape[3] in (64, 128) and bounds.dtype == dtype and bounds.is_contiguous()
-             and bounds.data_ptr() % 16 == 0,
-             "key bounds must be contiguous [pages, kv_heads, 2, head_dim] in the queries' dtype")
-    _require(bounds.is_cuda, "key bounds must be on a CUDA device")
-    _require(geometry is None or (shape[0], shape[1], shape[3]) == geometry[:3], "key bounds do not match the pool")
+    if (len(shape) != 4 or shape[2] != 2 or shape[3] not in (64, 128) or bounds.dtype != dtype or not bounds.is_contiguous()
+            or bounds.data_ptr() % 16):
+        raise ValueError("key bounds must be contiguous [pages, kv_heads, 2, head_dim] in the queries' dtype")
+    if not bounds.is_cuda:
+        raise ValueError("key bounds must be on a CUDA device")
+    if geometry is not None and (shape[0] != geometry[0] or shape[1] != geometry[1] or shape[3] != geometry[2]):
+        raise ValueError("key bounds do not match the pool")
 
 
 def update_key_bounds_int4(kv4_pool, key_bounds, block_table, seq_lens, *, new_tokens=1):
@@ -392,9 +405,9 @@ def update_key_bounds_int4(kv4_pool, key_bounds, block_table, seq_lens, *, new_t
              "new_tokens must be a non-negative integer")
     device = kv4_pool.get_device()
     _require(key_bounds.get_device() == device, _PAGED_DEVICE)
-    args, _ = _paged(device, block_table.shape[0], geometry, dtype, block_table, seq_lens, pool=kv4_pool, bounds=key_bounds,
-                     new_tokens=new_tokens)
-    _enqueue(_cabi().library().qf_int4_key_bounds, ctypes.byref(args), device=device)
+    args = _paged(device, block_table.shape[0], geometry, dtype, block_table, seq_lens, False, None, None, kv4_pool, key_bounds,
+                  None, new_tokens, 0, 0.0)
+    _enqueue(_cabi().library().qf_int4_key_bounds, (ctypes.byref(args),), device)
     return key_bounds
 
 
@@ -425,10 +438,11 @@ def select_kv_pages(q, key_bounds, block_table, seq_lens, *, num_pages, page_siz
     device = key_bounds.get_device()
     _require(q.get_device() == device, _PAGED_DEVICE)
     choice = _empty_choice(q.shape[0], kv_heads, num_pages, q.device)
+    args = _paged(device, q.shape[0], geometry, dtype, block_table, seq_lens, False, q, None, None, key_bounds, choice, 0,
+                  num_pages, 0.0)
     cabi = _cabi()
-    args, scratch = _paged(device, q.shape[0], geometry, dtype, block_table, seq_lens, q=q, bounds=key_bounds, choice=choice,
-                           take=num_pages, call=cabi.INT4_SELECT)
-    _enqueue(cabi.library().qf_select_kv_pages, ctypes.byref(args), device=device)
+    scratch = _scratch(args, cabi.INT4_SELECT, device, q)
+    _enqueue(cabi.library().qf_select_kv_pages, (ctypes.byref(args),), device)
     del scratch
     return choice
 
@@ -443,12 +457,12 @@ def sparse_decode_attention_int4(q, kv4_pool, key_bounds, block_table, seq_lens,
     _check_take(num_pages)
     device = kv4_pool.get_device()
     _require(q.get_device() == device and key_bounds.get_device() == device, _PAGED_DEVICE)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     choice = _empty_choice(q.shape[0], geometry[1], num_pages, q.device)
+    args = _paged(device, q.shape[0], geometry, dtype, block_table, seq_lens, False, q, out, kv4_pool, key_bounds, choice, 0,
+                  num_pages, geometry[2] ** -0.5 if scale is None else scale)
     cabi = _cabi()
-    args, scratch = _paged(device, q.shape[0], geometry, dtype, block_table, seq_lens, q=q, out=out, pool=kv4_pool,
-                           bounds=key_bounds, choice=choice, take=num_pages,
-                           scale=geometry[2] ** -0.5 if scale is None else scale, call=cabi.INT4_SPARSE)
-    _enqueue(cabi.library().qf_int4_sparse_decode_attention, ctypes.byref(args), device=device)
+    scratch = _scratch(args, cabi.INT4_SPARSE, device, q)
+    _enqueue(cabi.library().qf_int4_sparse_decode_attention, (ctypes.byref(args),), device)
     del scratch
     return out, *choice
