@@ -405,7 +405,7 @@ PagedInt4 over_selection(PagedInt4 p) {
 }
 
 int launch_select(const PagedInt4& p, int head_dim, int dtype, cudaStream_t stream) {
-  QF_REQUIRE(p.workspace != nullptr && p.workspace_bytes >= select_bytes(p), "the workspace holds %lld bytes, %lld are needed",
+  QF_REQUIRE((p.workspace != nullptr || select_bytes(p) == 0) && p.workspace_bytes >= select_bytes(p), "the workspace holds %lld bytes, %lld are needed",
              static_cast<long long>(p.workspace_bytes), static_cast<long long>(select_bytes(p)));
   const int rows = p.batch * p.kv_heads;
   QF_REQUIRE(rows <= 65535, "at most 65535 (sequence, KV head) rows choose pages in one call");

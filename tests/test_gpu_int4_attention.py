@@ -114,6 +114,38 @@ def test_empty_batch_and_infinite_values(package, cuda_device):
     assert torch.isnan(out[0, 6:]).all() and torch.isfinite(out[0, :6]).all() and torch.isfinite(out[1]).all()
 
 
+def test_tables_without_pages_and_pools_without_pages(package, cuda_device):
+    """A table of width 0 holds no token; a pool without pages has none to read."""
+    q, pool, table, lens = (t.to(cuda_device) for t in plain.make_cache([40, 20], seed=1))
+    limits = torch.zeros(pool.shape[0], 2, 2, 128, dtype=q.dtype, device=cuda_device)
+    out = package.paged_decode_attention_int4(q, pool, table[:, :0], lens)
+    assert (out == 0).all()
+    pages, held = package.select_kv_pages(q, limits, table[:, :0], lens, num_pages=3)
+    assert (pages == -1).all() and (held == 0).all()
+    out, pages, held = package.sparse_decode_attention_int4(q, pool, limits, table[:, :0], lens, num_pages=3)
+    assert (out == 0).all() and (pages == -1).all() and (held == 0).all()
+    package.update_key_bounds_int4(pool, limits, table[:, :0], lens, new_tokens=5)
+    assert package.cabi.device_status() == 0
+    out = package.paged_decode_attention_int4(q, pool[:0], table, lens)
+    assert (out == 0).all() and package.cabi.device_status() == 2
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.07, 3.0])
+def test_scales(package, cuda_device, scale):
+    q, pool, table, lens = plain.make_cache([0, 1, 33, 200, 700], seed=8)
+    _check(package, cuda_device, (q * 0.3).half(), pool, table, lens, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_more_rows_than_shared_memory_keeps(package, cuda_device, dtype):
+    """Thousands of rows, many of them empty: lengths come from global memory and threads take several rows."""
+    g = torch.Generator().manual_seed(1)
+    lengths = torch.randint(0, 40, (700,), generator=g).tolist() + [900, 0, 0, 0, 5]
+    q, pool, table, lens = plain.make_cache(lengths, dtype=dtype, dim=64, heads=4, group=2, seed=4)
+    out = _check(package, cuda_device, q, pool, table, lens)
+    assert (out[lens == 0] == 0).all()
+
+
 def test_pool_beyond_four_gigabytes(package, cuda_device):
     q, pool, table, lens = plain.make_cache([100, 333], seed=6)
     far = 2 ** 32 // (2 * 2560) + 1000
@@ -276,6 +308,30 @@ def test_same_bits_again_other_streams_and_two_graphs(package, cuda_device):
     torch.cuda.synchronize()
     for (_, out), b in zip(graphs, want):
         assert torch.equal(out, b)
+
+
+def test_two_captured_sparse_calls_side_by_side(package, cuda_device):
+    """Scratch and choices are each graph's own: replayed together they give what they give alone."""
+    cases = []
+    for seed, lengths in ((3, [4000, 900, 2500]), (4, [1500] * 6)):
+        q, pool, table, lens = plain.make_cache(lengths, seed=seed)
+        k, _ = plain.rows(pool, q.dtype)
+        limits = plain.bounds(k, table, lens, q.dtype, 10 ** 6, torch.zeros(pool.shape[0], 2, 2, 128, dtype=q.dtype))
+        cases.append(tuple(t.to(cuda_device) for t in (q, pool, limits, table, lens)))
+    alone = [package.sparse_decode_attention_int4(*c, num_pages=20) for c in cases]
+    graphs = []
+    for c in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outputs = package.sparse_decode_attention_int4(*c, num_pages=20)
+        graphs.append((graph, outputs, torch.cuda.Stream()))
+    for _ in range(30):
+        for graph, _, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (_, outputs, _), want in zip(graphs, alone):
+        assert all(torch.equal(a, b) for a, b in zip(outputs, want))
 
 
 def test_neighbouring_calls_do_not_race(package, cuda_device):

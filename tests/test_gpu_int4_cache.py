@@ -98,6 +98,27 @@ def test_write_forms_and_strides(package, cuda_device, dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_codes_of_quotients_between_two(package, cuda_device, dtype):
+    """Values on and beside the borders between two codes, and tiny, huge and equal ones: the kernel's quotients are
+    the correctly rounded ones, tie for tie."""
+    g = torch.Generator().manual_seed(2)
+    rows, heads, dim = 4096, 2, 128
+    info = torch.finfo(dtype)
+    step = torch.rand(rows, heads, dim // 32, 1, generator=g).mul(8).sub(4).exp()
+    low = torch.randn(rows, heads, dim // 32, 1, generator=g) * step * 20
+    x = low + step * (torch.randint(0, 31, (rows, heads, dim // 32, 32), generator=g) * 0.5)
+    x = x.flatten(-2).to(dtype)
+    x[:64] = (x[:64].float() * info.tiny * 4).to(dtype)           # down to subnormal steps
+    x[64:128] = (x[64:128].float().sign() * info.max * 0.25 * torch.rand(64, heads, dim, generator=g)).to(dtype)
+    x[128:140] = 0.0
+    k, v = x, x.flip(-1)
+    pool = torch.zeros(rows // 16, heads, 1, 20 * dim, dtype=torch.uint8)
+    plain.store_fast(pool, torch.arange(rows), k, v)
+    got = package.quantize_kv_pool_int4(*(t.to(cuda_device).view(rows // 16, 16, heads, dim) for t in (k, v)))
+    _same_cache(got.cpu(), pool, dtype)
+
+
 def test_valid_tokens_empty_calls_and_positions_past_the_table(package, cuda_device):
     g = torch.Generator().manual_seed(8)
     packed = torch.randn(6, 2048, generator=g).half().to(cuda_device)
