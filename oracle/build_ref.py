@@ -63,7 +63,7 @@ def build_ref(reference: Path | str | None = None, force: bool = False) -> Path 
     """Copy REFERENCE_FILES from the reference tree into oracle/_ref/.  Returns the
     directory, or None when neither the tree nor an earlier copy is present."""
     root = Path(reference) if reference is not None else DEFAULT_REFERENCE
-    if not root.is_dir():
+    if not any((root / relative).is_file() for relative in REFERENCE_FILES):  # no tree, or an empty mount point
         return REF_DIR if MANIFEST.is_file() else None
     entries = {}
     for relative in REFERENCE_FILES:
