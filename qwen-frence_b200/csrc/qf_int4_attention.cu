@@ -496,15 +496,16 @@ struct Row {
       }
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const uint32_t u0 = v0[w] >> 8, u1 = v1[w] >> 8;
+        // rows g of a product are codes 2 k, rows g + 8 the bytes with codes 2 k (low) and 2 k + 1
+        const uint32_t u0 = __byte_perm(v0[w], 0u, 0x4341u), u1 = __byte_perm(v1[w], 0u, 0x4341u);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           if constexpr (kCentred) {  // 7.5 in row w of an A that is zero elsewhere: one sum for all groups
             const uint32_t ones = g == w ? 0x47804780u : 0u;
             mma_f16(h[i], ones, 0u, ones, 0u, pb[i][w][0], pb[i][w][1]);
           }
-          mma_f16(o[i][2 * w], v0[w] & 0x000f000fu, v0[w] & 0x00f000f0u, v1[w] & 0x000f000fu, v1[w] & 0x00f000f0u, pb[i][w][0], pb[i][w][1]);
-          mma_f16(o[i][2 * w + 1], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, pb[i][w][0], pb[i][w][1]);
+          mma_f16(o[i][2 * w], v0[w] & 0x000f000fu, v0[w] & 0x00ff00ffu, v1[w] & 0x000f000fu, v1[w] & 0x00ff00ffu, pb[i][w][0], pb[i][w][1]);
+          mma_f16(o[i][2 * w + 1], u0 & 0x000f000fu, u0, u1 & 0x000f000fu, u1, pb[i][w][0], pb[i][w][1]);
         }
       }
     }
@@ -528,8 +529,10 @@ struct Row {
           if constexpr (kCentred) sum -= __shfl_sync(0xffffffffu, h[i][y], 4 * w + t);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
+            // rows g + 8 are code + 16 * next code
+            const float next = o[i][2 * w + k][2 + y] - o[i][2 * w + k][y];
             o[i][2 * w + k][y] = fmaf(o[i][2 * w + k][y], 16777216.f, sum);
-            o[i][2 * w + k][2 + y] = fmaf(o[i][2 * w + k][2 + y], 1048576.f, sum);
+            o[i][2 * w + k][2 + y] = fmaf(next, 1048576.f, sum);
           }
         }
       }
