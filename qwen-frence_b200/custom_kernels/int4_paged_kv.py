@@ -39,22 +39,19 @@ import torch
 TILE_TOKENS = 16
 MAX_GROUP = 16
 
-_cabi_module = None
-
-
-def _cabi():
+def _load_cabi():
     """The ctypes binding, loaded by path so this file works under any module name."""
-    global _cabi_module
-    if _cabi_module is None:
-        module = sys.modules.get("qf_hotpath_cabi")
-        if module is None:
-            path = Path(__file__).resolve().parents[1] / "_cabi.py"
-            spec = importlib.util.spec_from_file_location("qf_hotpath_cabi", path)
-            module = importlib.util.module_from_spec(spec)
-            sys.modules["qf_hotpath_cabi"] = module
-            spec.loader.exec_module(module)
-        _cabi_module = module
-    return _cabi_module
+    module = sys.modules.get("qf_hotpath_cabi")
+    if module is None:
+        path = Path(__file__).resolve().parents[1] / "_cabi.py"
+        spec = importlib.util.spec_from_file_location("qf_hotpath_cabi", path)
+        module = importlib.util.module_from_spec(spec)
+        sys.modules["qf_hotpath_cabi"] = module
+        spec.loader.exec_module(module)
+    return module
+
+
+_cabi = _load_cabi()
 
 
 def _require(condition, message):
@@ -97,14 +94,13 @@ def _index_code(tensor, what):
 
 def _enqueue(function, arguments, device):
     """One library call on the current stream of CUDA device number `device`, which is current meanwhile."""
-    cabi = _cabi_module
     if torch.cuda.current_device() == device:
-        status = function(*arguments, cabi.raw_stream(device))
+        status = function(*arguments, _cabi.raw_stream(device))
     else:
         with torch.cuda.device(device):
-            status = function(*arguments, cabi.raw_stream(device))
+            status = function(*arguments, _cabi.raw_stream(device))
     if status:
-        cabi.check(status)
+        _cabi.check(status)
 
 
 def empty_kv_pool_int4(num_pages, kv_heads, head_dim, *, page_size=16, device=None):
@@ -127,40 +123,40 @@ def _write(pool, geometry, pointers, strides, like, positions, slot_mapping, *, 
     """Check what every write shares, fill qf_int4_write_args and enqueue on the current stream.
     `pointers` of q, k, v and q_out; `strides` of their rows, heads and channels, twelve numbers."""
     pages, kv_heads, dim, page_size = geometry
-    cabi = _cabi()
     device = pool.get_device()
     dtype = _element_code(like.dtype)
-    _require(like.get_device() == device, "the 4-bit cache write needs CUDA tensors of one device")
-    position_at = position_stride = position_code = 0
+    position_at = position_stride = position_code = slot_at = slot_stride = slot_code = table_at = table_positions = valid_at = 0
+    one_device = like.get_device() == device
     if positions is not None:
-        _require(positions.get_device() == device, "the 4-bit cache write needs CUDA tensors of one device")
+        one_device = one_device and positions.get_device() == device
         if positions.dtype is torch.float32 and rope_table is None:
-            position_code = cabi.INDEX_F32
+            position_code = _cabi.INDEX_F32
         else:
             position_code = _index_code(positions, "positions")
-        position_at, position_stride = positions.data_ptr(), positions.stride(0)
-    slot_at = slot_stride = slot_code = 0
+        position_at = positions.data_ptr()
+        position_stride, = positions.stride()
     if slot_mapping is not None:
-        _require(slot_mapping.get_device() == device, "the 4-bit cache write needs CUDA tensors of one device")
-        slot_at, slot_stride = slot_mapping.data_ptr(), slot_mapping.stride(0)
+        one_device = one_device and slot_mapping.get_device() == device
         slot_code = _index_code(slot_mapping, "slot mapping")
-    table_at = table_positions = 0
+        slot_at = slot_mapping.data_ptr()
+        slot_stride, = slot_mapping.stride()
     if rope_table is not None:
-        table_positions = rope_table.shape[0]
-        _require(rope_table.shape == (table_positions, dim // 2, 2) and table_positions >= 1
-                 and rope_table.dtype is torch.float32 and rope_table.is_contiguous() and rope_table.data_ptr() % 16 == 0,
-                 "rope_table must be contiguous, 16-byte aligned float32 [positions, head_dim / 2, 2]")
-        _require(rope_table.get_device() == device, "the 4-bit cache write needs CUDA tensors of one device")
-        table_at = rope_table.data_ptr()
-    valid_at = None
+        shape = rope_table.shape
+        table_positions, table_at = shape[0], rope_table.data_ptr()
+        if (len(shape) != 3 or table_positions < 1 or shape[1] * 2 != dim or shape[2] != 2 or rope_table.dtype is not torch.float32
+                or not rope_table.is_contiguous() or table_at % 16):
+            raise ValueError("rope_table must be contiguous, 16-byte aligned float32 [positions, head_dim / 2, 2]")
+        one_device = one_device and rope_table.get_device() == device
     if valid_tokens is not None:
-        _require(valid_tokens.dtype is torch.int32 and valid_tokens.numel() == 1 and valid_tokens.get_device() == device,
-                 "valid_tokens must be a CUDA int32 scalar")
+        if valid_tokens.dtype is not torch.int32 or valid_tokens.numel() != 1 or valid_tokens.get_device() != device:
+            raise ValueError("valid_tokens must be a CUDA int32 scalar")
         valid_at = valid_tokens.data_ptr()
-    args = cabi.Int4WriteArgs(
+    if not one_device:
+        raise ValueError("the 4-bit cache write needs CUDA tensors of one device")
+    args = _cabi.pack_int4_write(
         *pointers, *strides, position_at, position_stride, slot_at, slot_stride, table_at, pool.data_ptr(), pages, valid_at,
         rows, q_heads, kv_heads, dim, page_size, dtype, position_code, slot_code, table_positions, base)
-    _enqueue(cabi.library().qf_int4_rope_kv_write, (ctypes.byref(args),), device)
+    _enqueue(_cabi.library().qf_int4_rope_kv_write, (args,), device)
 
 
 def packed_qkv_rope_cache_int4(
@@ -176,13 +172,15 @@ def packed_qkv_rope_cache_int4(
         _require(packed.shape[1] == 1, "packed QKV must have one decode token per row")
         packed = packed[:, 0, :]
     geometry = _, kv_heads, dim, _ = _check_pool(kv4_pool)
-    _require(q_heads >= 1, "q_heads must be positive")
-    _require(packed.ndim == 2 and packed.shape[1] == (q_heads + 2 * kv_heads) * dim,
-             "expected packed QKV shape (rows, (q_heads + 2 * kv_heads) * head_dim)")
-    rows = packed.shape[0]
-    _require(positions.shape == (rows,) and slot_mapping.shape == (rows,),
-             "positions and slots must contain one value per row")
-    q = torch.empty((rows, q_heads, dim), device=packed.device, dtype=packed.dtype)
+    if q_heads < 1:
+        raise ValueError("q_heads must be positive")
+    shape = packed.shape
+    if len(shape) != 2 or shape[1] != (q_heads + 2 * kv_heads) * dim:
+        raise ValueError("expected packed QKV shape (rows, (q_heads + 2 * kv_heads) * head_dim)")
+    rows = shape[0]
+    if positions.shape != (rows,) or slot_mapping.shape != (rows,):
+        raise ValueError("positions and slots must contain one value per row")
+    q = torch.empty(rows, q_heads, dim, device=packed.device, dtype=packed.dtype)
     if rows == 0:
         return q
     row_stride, col_stride = packed.stride()
@@ -200,7 +198,7 @@ def _write_heads(q, k, v, positions, slot_mapping, kv4_pool, geometry, token_dim
     _require(q.get_device() == k.get_device() == v.get_device(), "the 4-bit cache write needs CUDA tensors of one device")
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if rotate_q else q
     strides = tuple(t.stride(n) for t in (q, k, v, out) for n in (token_dim, 1, 3))
-    _write(kv4_pool, geometry, (q.data_ptr() if rotate_q else None, k.data_ptr(), v.data_ptr(), out.data_ptr() if rotate_q else None),
+    _write(kv4_pool, geometry, (q.data_ptr() if rotate_q else 0, k.data_ptr(), v.data_ptr(), out.data_ptr() if rotate_q else 0),
            strides, k, positions, slot_mapping, rows=k.shape[token_dim], q_heads=q.shape[1] if rotate_q else 0, base=base,
            rope_table=rope_table)
     return out
@@ -249,7 +247,7 @@ def quantize_kv_pool_int4(k_pool, v_pool):
     _require(k_pool.is_cuda and v_pool.device == k_pool.device, "K/V pools must share one CUDA device")
     pool = empty_kv_pool_int4(pages, kv_heads, dim, page_size=page_size, device=k_pool.device)
     _require(v_pool.dtype == k_pool.dtype, "K/V pools must share FP16 or BF16 dtype")
-    _write(pool, (pages, kv_heads, dim, page_size), (None, k_pool.data_ptr(), v_pool.data_ptr(), None),
+    _write(pool, (pages, kv_heads, dim, page_size), (0, k_pool.data_ptr(), v_pool.data_ptr(), 0),
            (kv_heads * dim, dim, 1) * 4, k_pool, None, None, rows=pages * page_size, q_heads=0, base=1.0, rope_table=None)
     return pool
 
@@ -258,21 +256,24 @@ def _read(kv4_pool, slots, rows, dtype):
     """Rows at `slots` = (address, index code, stride) as K and V [rows, kv_heads, D]."""
     pages, kv_heads, dim, page_size = _check_pool(kv4_pool)
     code = _element_code(dtype)
-    both = torch.empty((2, rows, kv_heads, dim), dtype=dtype, device=kv4_pool.device)
-    at = both.data_ptr()
-    _enqueue(_cabi().library().qf_int4_read_rows,
-             (kv4_pool.data_ptr(), pages, page_size, kv_heads, dim, code, *slots, rows, at, at + 2 * rows * kv_heads * dim),
+    k = torch.empty(rows, kv_heads, dim, dtype=dtype, device=kv4_pool.device)
+    v = torch.empty_like(k)
+    _enqueue(_cabi.library().qf_int4_read_rows,
+             (kv4_pool.data_ptr(), pages, page_size, kv_heads, dim, code, *slots, rows, k.data_ptr(), v.data_ptr()),
              kv4_pool.get_device())
-    return both.unbind(0)
+    return k, v
 
 
 def read_kv_int4(kv4_pool, slot_mapping, *, dtype=None):
     """Rows of the cache at a list of slots as (k, v), both [n, Hkv, D] in `dtype` (that of the
     writes; default float16).  A slot outside the pool, -1 for one, gives a row of zeros."""
-    _require(slot_mapping.ndim == 1, "slot mapping must be a list of slots")
-    _require(slot_mapping.get_device() == kv4_pool.get_device(), "pool and slots must share one CUDA device")
-    slots = (slot_mapping.data_ptr(), _index_code(slot_mapping, "slot mapping"), slot_mapping.stride(0))
-    return _read(kv4_pool, slots, slot_mapping.shape[0], torch.float16 if dtype is None else dtype)
+    shape = slot_mapping.shape
+    if len(shape) != 1:
+        raise ValueError("slot mapping must be a list of slots")
+    if slot_mapping.get_device() != kv4_pool.get_device():
+        raise ValueError("pool and slots must share one CUDA device")
+    slots = (slot_mapping.data_ptr(), _index_code(slot_mapping, "slot mapping"), *slot_mapping.stride())
+    return _read(kv4_pool, slots, shape[0], torch.float16 if dtype is None else dtype)
 
 
 def dequantize_kv_pool_int4(kv4_pool, dtype=None):
@@ -289,25 +290,10 @@ _workspace_sizes = {}
 _PAGED_DEVICE = "queries, pool, key bounds, page table and lengths must share one CUDA device"
 
 
-def _scratch(args, call, device, like):
-    """Scratch of one call: a torch allocation, so it is the stream's, and a captured graph's own."""
-    key = (call, device, args.batch, args.q_heads, args.kv_heads, args.head_dim, args.page_size, args.table_width, args.take)
-    need = _workspace_sizes.get(key)
-    if need is None:
-        cabi, size = _cabi(), ctypes.c_int64()
-        with torch.cuda.device(device):
-            cabi.check(cabi.library().qf_paged_int4_workspace(ctypes.byref(args), call, ctypes.byref(size)))
-        if len(_workspace_sizes) >= 4096:
-            _workspace_sizes.clear()
-        need = _workspace_sizes[key] = size.value
-    scratch = torch.empty(need, dtype=torch.uint8, device=like.device)
-    args.workspace = scratch.data_ptr()
-    args.workspace_bytes = need
-    return scratch
-
-
-def _paged(device, batch, geometry, dtype, block_table, seq_lens, per_head, q, out, pool, bounds, choice, new_tokens, take, scale):
-    """Check table and lengths and fill qf_paged_int4_args (no scratch yet)."""
+def _run(function, call, device, batch, geometry, dtype, block_table, seq_lens, per_head, q, out, pool, bounds, choice, new_tokens,
+         take, scale):
+    """Check table and lengths, fill qf_paged_int4_args, add the scratch of `call` (None: it has none) and
+    enqueue.  The scratch is a torch allocation, so it is the stream's, and a captured graph's own."""
     pages, kv_heads, dim, page_size = geometry
     t_shape = block_table.shape
     if per_head and len(t_shape) == 3:
@@ -315,16 +301,17 @@ def _paged(device, batch, geometry, dtype, block_table, seq_lens, per_head, q, o
             raise ValueError("a table and lengths per KV head have shapes [batch, kv_heads, pages] and [batch, kv_heads]")
         t_sb, t_sh, t_sp = block_table.stride()
         l_sb, l_sh = seq_lens.stride()
+        width = t_shape[2]
     else:
         if len(t_shape) != 2 or t_shape[0] != batch or seq_lens.shape != (batch,):
             raise ValueError("batch dimensions must match")
         t_sb, t_sp = block_table.stride()
         l_sb, = seq_lens.stride()
         t_sh = l_sh = 0
+        width = t_shape[1]
     if block_table.get_device() != device or seq_lens.get_device() != device:
         raise ValueError(_PAGED_DEVICE)
-    q_at = o_at = pages_at = held_at = None
-    q_heads = q_sb = q_sh = o_sb = 0
+    q_at = o_at = pages_at = held_at = q_heads = q_sb = q_sh = o_sb = scratch_at = scratch_bytes = 0
     if q is not None:
         q_at, q_heads = q.data_ptr(), q.shape[1]
         q_sb, q_sh, _ = q.stride()
@@ -332,11 +319,27 @@ def _paged(device, batch, geometry, dtype, block_table, seq_lens, per_head, q, o
         o_at, o_sb = out.data_ptr(), q_heads * dim
     if choice is not None:
         pages_at, held_at = choice[0].data_ptr(), choice[1].data_ptr()
-    return _cabi().PagedInt4Args(
-        q_at, o_at, None if pool is None else pool.data_ptr(), None if bounds is None else bounds.data_ptr(),
-        block_table.data_ptr(), seq_lens.data_ptr(), None, pages_at, held_at, q_sb, q_sh, o_sb, dim, t_sb, t_sh, t_sp, l_sb, l_sh,
-        pages, t_shape[-1], 0, batch, q_heads, kv_heads, dim, page_size, dtype, _index_code(block_table, "page table"),
-        _index_code(seq_lens, "lengths"), new_tokens, take, scale)
+
+    def fill():
+        return _cabi.pack_paged_int4(
+            q_at, o_at, 0 if pool is None else pool.data_ptr(), 0 if bounds is None else bounds.data_ptr(),
+            block_table.data_ptr(), seq_lens.data_ptr(), scratch_at, pages_at, held_at, q_sb, q_sh, o_sb, dim, t_sb, t_sh, t_sp,
+            l_sb, l_sh, pages, width, scratch_bytes, batch, q_heads, kv_heads, dim, page_size, dtype,
+            _index_code(block_table, "page table"), _index_code(seq_lens, "lengths"), new_tokens, take, scale)
+
+    if call is not None:
+        key = (call, device, batch, q_heads, kv_heads, dim, page_size, width, take)
+        scratch_bytes = _workspace_sizes.get(key)
+        if scratch_bytes is None:
+            scratch_bytes, size = 0, ctypes.c_int64()
+            with torch.cuda.device(device):
+                _cabi.check(_cabi.library().qf_paged_int4_workspace(fill(), call, ctypes.byref(size)))
+            if len(_workspace_sizes) >= 4096:
+                _workspace_sizes.clear()
+            scratch_bytes = _workspace_sizes[key] = size.value
+        scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=block_table.device)
+        scratch_at = scratch.data_ptr()
+    _enqueue(function, (fill(),), device)
 
 
 def _check_query(q, geometry):
@@ -371,12 +374,8 @@ def paged_decode_attention_int4(q, kv4_pool, block_table, seq_lens, *, scale=Non
     if q.get_device() != device:
         raise ValueError(_PAGED_DEVICE)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    args = _paged(device, q.shape[0], geometry, dtype, block_table, seq_lens, True, q, out, kv4_pool, None, None, 0, 0,
-                  geometry[2] ** -0.5 if scale is None else scale)
-    cabi = _cabi()
-    scratch = _scratch(args, cabi.INT4_ATTENTION, device, q)
-    _enqueue(cabi.library().qf_int4_decode_attention, (ctypes.byref(args),), device)
-    del scratch
+    _run(_cabi.library().qf_int4_decode_attention, _cabi.INT4_ATTENTION, device, q.shape[0], geometry, dtype, block_table, seq_lens,
+         True, q, out, kv4_pool, None, None, 0, 0, geometry[2] ** -0.5 if scale is None else scale)
     return out
 
 
@@ -405,9 +404,8 @@ def update_key_bounds_int4(kv4_pool, key_bounds, block_table, seq_lens, *, new_t
              "new_tokens must be a non-negative integer")
     device = kv4_pool.get_device()
     _require(key_bounds.get_device() == device, _PAGED_DEVICE)
-    args = _paged(device, block_table.shape[0], geometry, dtype, block_table, seq_lens, False, None, None, kv4_pool, key_bounds,
-                  None, new_tokens, 0, 0.0)
-    _enqueue(_cabi().library().qf_int4_key_bounds, (ctypes.byref(args),), device)
+    _run(_cabi.library().qf_int4_key_bounds, None, device, block_table.shape[0], geometry, dtype, block_table, seq_lens, False,
+         None, None, kv4_pool, key_bounds, None, new_tokens, 0, 0.0)
     return key_bounds
 
 
@@ -417,8 +415,8 @@ def _check_take(num_pages):
 
 
 def _empty_choice(batch, kv_heads, num_pages, device):
-    return (torch.empty((batch, kv_heads, num_pages), dtype=torch.int32, device=device),
-            torch.empty((batch, kv_heads), dtype=torch.int32, device=device))
+    return (torch.empty(batch, kv_heads, num_pages, dtype=torch.int32, device=device),
+            torch.empty(batch, kv_heads, dtype=torch.int32, device=device))
 
 
 def select_kv_pages(q, key_bounds, block_table, seq_lens, *, num_pages, page_size=16):
@@ -438,12 +436,8 @@ def select_kv_pages(q, key_bounds, block_table, seq_lens, *, num_pages, page_siz
     device = key_bounds.get_device()
     _require(q.get_device() == device, _PAGED_DEVICE)
     choice = _empty_choice(q.shape[0], kv_heads, num_pages, q.device)
-    args = _paged(device, q.shape[0], geometry, dtype, block_table, seq_lens, False, q, None, None, key_bounds, choice, 0,
-                  num_pages, 0.0)
-    cabi = _cabi()
-    scratch = _scratch(args, cabi.INT4_SELECT, device, q)
-    _enqueue(cabi.library().qf_select_kv_pages, (ctypes.byref(args),), device)
-    del scratch
+    _run(_cabi.library().qf_select_kv_pages, _cabi.INT4_SELECT, device, q.shape[0], geometry, dtype, block_table, seq_lens, False,
+         q, None, None, key_bounds, choice, 0, num_pages, 0.0)
     return choice
 
 
@@ -459,10 +453,6 @@ def sparse_decode_attention_int4(q, kv4_pool, key_bounds, block_table, seq_lens,
     _require(q.get_device() == device and key_bounds.get_device() == device, _PAGED_DEVICE)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     choice = _empty_choice(q.shape[0], geometry[1], num_pages, q.device)
-    args = _paged(device, q.shape[0], geometry, dtype, block_table, seq_lens, False, q, out, kv4_pool, key_bounds, choice, 0,
-                  num_pages, geometry[2] ** -0.5 if scale is None else scale)
-    cabi = _cabi()
-    scratch = _scratch(args, cabi.INT4_SPARSE, device, q)
-    _enqueue(cabi.library().qf_int4_sparse_decode_attention, (ctypes.byref(args),), device)
-    del scratch
+    _run(_cabi.library().qf_int4_sparse_decode_attention, _cabi.INT4_SPARSE, device, q.shape[0], geometry, dtype, block_table,
+         seq_lens, False, q, out, kv4_pool, key_bounds, choice, 0, num_pages, geometry[2] ** -0.5 if scale is None else scale)
     return out, *choice

@@ -31,6 +31,13 @@ def test_structs_match_c_layout(package, tmp_path):
             assert int(reported[f"{struct}.{name}"]) == getattr(cls, name).offset, (struct, name)
 
 
+def test_packed_arguments_are_the_structures_bytes(package):
+    cabi = package.cabi
+    for cls, pack in ((cabi.Int4WriteArgs, cabi.pack_int4_write), (cabi.PagedInt4Args, cabi.pack_paged_int4)):
+        values = [(i * 37 + 5) / 4 if kind in (ctypes.c_float, ctypes.c_double) else i * 1000003 + 1 for i, (_, kind) in enumerate(cls._fields_)]
+        assert pack(*values) == bytes(cls(*values)) and len(pack(*values)) == ctypes.sizeof(cls)
+
+
 def _write_args(cabi, **changes):
     args = cabi.Int4WriteArgs()
     values = dict(rows=1, q_heads=0, kv_heads=2, head_dim=128, page_size=16, dtype=0, k=16, v=16, pool=16, num_pages=4, base=1e6)
