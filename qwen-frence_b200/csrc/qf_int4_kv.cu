@@ -33,20 +33,22 @@ struct WriteParams {
   int pos_dtype, slot_dtype;
 };
 
-constexpr int kWriteThreads = 256;
+constexpr int kWriteThreads = 128;
 
 // Where the angles of a call come from.
 enum : int { kNoRope, kTable, kAngles };
 
 // Rows and their segments (heads) are laid end to end: a segment takes D / 16 threads, each with
-// the eight channels at d0 and the eight they rotate with at d0 + D / 2, so a CTA of 256 covers
-// two rows of 12 + 2 + 2 heads and no thread idles.  A group of 32 channels is four neighbouring
-// threads, whose extremes meet in two shuffles.  A thread fetches its cosines and sines from the
-// table itself (a row's 14 rotated heads hit the first level cache; passing them through shared
-// memory instead costs a barrier behind two dependent loads); without a table the CTA computes
-// each once and shares it.
+// the eight channels at d0 and the eight they rotate with at d0 + D / 2, so a CTA of 128 covers a row
+// of 12 + 2 + 2 heads and no thread idles.  A group of 32 channels is four neighbouring threads, whose
+// extremes meet in two shuffles.  A thread fetches its cosines and sines from the table itself (a
+// row's 14 rotated heads hit the first level cache; passing them through shared memory instead costs
+// a barrier behind two dependent loads, 28 -> 22 us for 8192 rows); without a table the CTA computes
+// each once and shares it.  Bound by the latency of position -> table -> row and by issue: 8192 rows of
+// 12 + 2 + 2 x 128 take 17 us, 64 MB at 3.8 TB/s; with CTAs of 256 20 us, of 512 23 us, and with 12
+// CTAs an SM (40 registers) instead of 16 (32) 18 us.
 template <typename T, int D, bool VEC, int ROPE>
-__global__ void __launch_bounds__(kWriteThreads) int4_write_kernel(const WriteParams p, const __grid_constant__ InvFreqTable freq) {
+__global__ void __launch_bounds__(kWriteThreads, ROPE == kAngles ? 12 : 16) int4_write_kernel(const WriteParams p, const __grid_constant__ InvFreqTable freq) {
   constexpr int kHalf = D / 2, kLanes = D / 16, W = D / kInt4Group;
   release_dependents();
   dependency_wait();
@@ -214,16 +216,18 @@ __device__ __forceinline__ void load_elements(const uint8_t* at, float (&x)[W]) 
 
 // Rows at a list of slots as 16-bit K and V.  Four threads a row and head, eight channels of every
 // group each: seven loads bring a thread's D / 2 values, and its stores are 16 bytes beside its
-// neighbours'.  A slot outside the pool gives a row of zeros.
+// neighbours' (16 threads a row, each with its own slot and addresses, were bound by those: 40 us for
+// 131072 rows of 2 x 128).  Bound by the stores: the 177 MB take 34 us, 5.2 TB/s.  A slot outside the
+// pool gives a row of zeros.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) int4_read_kernel(const uint8_t* __restrict__ pool, const void* __restrict__ slots,
+__global__ void __launch_bounds__(128) int4_read_kernel(const uint8_t* __restrict__ pool, const void* __restrict__ slots,
                                                         int slot_dtype, int64_t slot_stride, int rows, int64_t num_slots,
                                                         const Divisor kv_heads, const Divisor page_size,
                                                         T* __restrict__ k_out, T* __restrict__ v_out) {
   constexpr int W = D / kInt4Group;
   release_dependents();
   dependency_wait();
-  const uint32_t segment = blockIdx.x * 64 + threadIdx.x / 4;
+  const uint32_t segment = blockIdx.x * 32 + threadIdx.x / 4;
   const int t = threadIdx.x % 4;
   const int row = quotient(segment, kv_heads);
   const int head = segment - row * kv_heads.d;
@@ -373,12 +377,12 @@ int qf_int4_read_rows(const void* pool, int64_t num_pages, int32_t page_size, in
   QF_REQUIRE(pool && k_out && v_out, "pool, k_out and v_out must not be null");
   QF_REQUIRE(aligned16(pool) && aligned16(k_out) && aligned16(v_out), "pool and outputs must be 16-byte aligned");
   QF_REQUIRE(rows < (1LL << 31) / kv_heads - 256, "too many rows in one call");
-  const dim3 grid(static_cast<unsigned>((rows * kv_heads + 63) / 64));
+  const dim3 grid(static_cast<unsigned>((rows * kv_heads + 31) / 32));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const uint8_t* bytes = static_cast<const uint8_t*>(pool);
   cudaError_t err = cudaSuccess;
 #define QF_LAUNCH_READ(T, D)                                                                                       \
-  err = launch_chained(int4_read_kernel<T, D>, grid, dim3(256), 0, s, bytes, slots, static_cast<int>(slot_dtype),  \
+  err = launch_chained(int4_read_kernel<T, D>, grid, dim3(128), 0, s, bytes, slots, static_cast<int>(slot_dtype),  \
                        slot_stride, static_cast<int>(rows), num_pages * page_size, make_divisor(kv_heads),         \
                        make_divisor(page_size), static_cast<T*>(k_out), static_cast<T*>(v_out))
   if (dtype == QF_DTYPE_F16) {
