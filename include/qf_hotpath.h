@@ -594,7 +594,8 @@ int qf_int4_key_bounds(const qf_paged_int4_args* args, void* stream);
  * page of the sequence, a NaN above every number).  page_table: their ids in the sequence's
  * order, the newest last, -1 behind them when the sequence has fewer; page_lens: the tokens
  * they hold -- a block table and lengths with head strides for qf_int4_decode_attention.  A
- * page id outside the pool scores below every other.  Table and lengths are those of the
+ * page id outside the pool scores below every other (one that 32 bits do not hold is -1 in
+ * page_table).  Table and lengths are those of the
  * sequences.  batch * kv_heads at most 65535.  Ends with qf_order_next_launch(). */
 int qf_select_kv_pages(const qf_paged_int4_args* args, void* stream);
 

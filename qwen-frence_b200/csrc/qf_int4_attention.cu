@@ -9,17 +9,31 @@
 // q carries the 1/16.  One AND makes two matrix elements.  Steps meet the fp32 sums of a group,
 // floors are one more product.  With p = exp2(s - offset) and V codes m, steps c, floors e,
 //     o[d, h] = sum_t (p[t, h] c[t, w(d)]) m[t, d] + sum_t p[t, h] e[t, w(d)]
-// where p c is rounded to fp16 (2^-11 of a weight; the products and sums are fp32).  The offset
-// is the running maximum of s plus that of log2(c) less 10, so p c stays between 2^-14 and 2^15
-// for all weights down to 2^-24 of the largest, whatever the magnitude of V; it is raised, and the
-// sums rescaled, only when a score or a step exceeds what the last offset allows by 2^4.
+// where p c is rounded to fp16 (2^-11 of a weight at most; products and sums are fp32).  The offset is
+// the running maximum of s, plus the exponent of the largest c, less 10, so that p c stays below 2^15
+// and keeps fp16's precision down to 2^-24 of the largest weight, whatever the magnitude of V; it is
+// raised, and the sums rescaled, only when a score or a step exceeds what the last offset allows by 2^4.
 //
-// Work.  Rows are laid end to end as tiles and every CTA takes an equal share of them, every warp
-// of the CTA an equal share of that, whatever rows it covers.  A warp streams its tiles, 20 * D
-// contiguous bytes each, through a ring of bulk copies of its own; warps share nothing until
-// their tiles are done.  A row that one warp holds whole is written from its registers; what the
-// warps of a CTA hold of one row is summed at the CTA's end, and rows that span CTAs by a second
-// kernel, in the order of the tiles: the same call gives the same bits.
+// Work.  Rows are laid end to end as units of two tiles and every CTA, one an SM, takes an equal share
+// of them, every warp of the CTA an equal share of that, whatever rows it covers.  A warp streams its
+// units, 2 x 20 * D contiguous bytes each, through a ring of its own with cp.async (as bulk copies with
+// a barrier a stage, the same ring took 125 instructions more a unit and 7 % more time at D = 64); warps
+// share nothing until their units are done.  A row that one warp holds whole is written from its
+// registers; what the warps of a CTA hold of one row is summed at the CTA's end, and rows that span
+// CTAs by a second kernel, in the order of the tiles: the same call gives the same bits.  Table and
+// lengths are read while the kernel in front drains, unless it writes them.
+//
+// Bound.  The cache's 5 bits a channel come in at the memory's rate only if the SM spends no more than
+// 110 cycles on a tile of D = 128 (55 at D = 64); it issues about 250 (200) instructions a tile, a third
+// of them the masks and shifts that take codes apart, on four schedulers of which each is busy six
+// cycles in ten.  With all tiles in one page, that is with no memory to wait for, calls take 7 % less
+// time, so issue and dependences bound it, and for short calls the way to the first tile (lengths, table,
+// tile: 3 us) and the two launches.  64 sequences of 129..4097 tokens, 12 heads on 2 of 128: 20 us, 42 MB,
+// 2.1 TB/s; 256 of 64..4096, 16 on 4 of 64: 49 us, 172 MB, 3.5 TB/s; one of 513: 7.7 us.
+// Warps an SM, D = 128: 8 take 22 us for the first, 10 22.3, 12 20.0, 14 20.9, 16 21.2 (from 13 on the
+// registers no longer hold a row: 168 against 128 a thread); D = 64: 12 take 54 us, 16 52, 20 54.
+// Taking the next unit's scores beside this one's values gives the schedulers two chains to choose from
+// and cost 3 to 5 %; V words rotated so that no two lanes meet in a bank changed nothing.
 #include <algorithm>
 #include <atomic>
 
@@ -39,7 +53,7 @@ struct Shape {
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kTileBytes = 20 * D;
   static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = 204 * 1024 / kWarps / kStageBytes;  // of a warp's ring: one less in flight
+  static constexpr int kStages = 204 * 1024 / kWarps / kStageBytes;  // of a warp's ring, one less in flight: D 128 3 or 5, D 64 5 or 10
   static constexpr int kRing = kStages * kStageBytes;
   static constexpr int kHeads = 8 * NT;        // query heads a row has room for
   static constexpr int kStride = D + 4;        // floats between heads of a piece: its float4 stores miss no bank
@@ -352,7 +366,7 @@ struct Row {
   __device__ __forceinline__ void raise(const float (&x)[NT][8], float magnitude, int left, int g) {
     magnitude = warp_max(magnitude);
     const int above = max(-60, (__float_as_int(magnitude) >> 23) - 126);  // magnitude < 2^above
-    const int next = max(e, min(above, 100));
+    const int next = max(e, min(above, 127));
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
 #pragma unroll
@@ -680,20 +694,15 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
 
   Requests ahead{};
   if (units > 0) {
-    {
-      const int2 found = find_rows(s_shares, first, lane);
-      ahead.row = found.x * chunk;
-      int before = first - found.y;
-      const int rows = p.batch * p.kv_heads;
-      while (ahead.row < rows) {
-        const int in_row = (tokens_of(p, s_shares, ahead.row) + kUnit - 1) / kUnit;
-        if (before < in_row) break;
-        before -= in_row;
-        ++ahead.row;
-      }
-      ahead.unit = before;
-      ahead.left = units;
+    const int2 found = find_rows(s_shares, first, lane);
+    int before = first - found.y;
+    for (ahead.row = found.x * chunk; ahead.row < p.batch * p.kv_heads; ++ahead.row) {
+      const int in_row = (tokens_of(p, s_shares, ahead.row) + kUnit - 1) / kUnit;
+      if (before < in_row) break;
+      before -= in_row;
     }
+    ahead.unit = before;
+    ahead.left = units;
   }
   int id = ahead.row, in_row = ahead.unit;  // of the unit at hand
   if (units > 0) ahead.refill(p, s_shares, lane);
@@ -736,13 +745,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
     const uint8_t* at = ring;
     while (done < units) {
       int tokens = 0;
-      while (id < p.batch * p.kv_heads) {
+      for (; id < p.batch * p.kv_heads; ++id, in_row = 0) {
         tokens = tokens_of(p, s_shares, id);
         if (in_row * kUnit < tokens) break;
-        ++id, in_row = 0;
       }
+      if (id >= p.batch * p.kv_heads) break;  // lengths that change under a call must not lead it out of the batch
       const int in_all = (tokens + kUnit - 1) / kUnit;
-      const int n = max(1, min(in_all - in_row, units - done));  // lengths that change under a call must not hang it
+      const int n = min(in_all - in_row, units - done);
       if (done > 0) row.load(p, id, group, lane, queries);
       row.start(p, queries, lane);
       const bool starts = in_row == 0, ends = in_row + n >= in_all;
@@ -773,6 +782,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
       }
       in_row += n;
     }
+    copies_wait<0>();
   }
   __syncthreads();
 

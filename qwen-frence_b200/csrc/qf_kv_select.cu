@@ -85,11 +85,14 @@ __device__ __forceinline__ float max2_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// A CTA of four warps takes four tiles: a page of four, or two of two, four of one.  A lane holds
-// eight channels of 16 / (32 / (D / 8)) tokens of its warp's tile, all loaded at once; two tokens a
-// step of the three-operand minimum and maximum.  A page of more tiles is its warps' in turn.
-// Rounding to T is monotone and comes once, after the warps of a page have met.
-constexpr int kBoundWarps = 4;
+// A warp takes a page, or four warps a page of kManyTiles and more; a lane holds eight channels of
+// 16 / (32 / (D / 8)) tokens of a tile, all loaded at once, and two tokens a step of the
+// three-operand minimum and maximum.  Rounding to T is monotone and comes once, after the warps of a
+// page have met.  Bound by issue, 25 instructions an eight codes: 16 prompts of 4096..8192 tokens
+// (2 x 128, pages of 64, 16 MB) take 10.7 us, a step's newest pages of 64 sequences 2.3 us.  Four warps
+// a page against one, the same prompts: pages of 64 tokens 14.8 and 10.7 us, of 128 12.0 and 15.5, of
+// 256 11.1 and 22.7.
+constexpr int kBoundWarps = 4, kManyTiles = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kBoundWarps) key_bounds_kernel(const PagedInt4 p, const Divisor by_each, int warps_each) {
   constexpr int W = D / kInt4Group, kWords = D / 8, kStep = 32 / kWords, kTokens = kInt4Tile / kStep;
@@ -283,6 +286,9 @@ __global__ void __launch_bounds__(128) page_score_kernel(const PagedInt4 p, uint
   }
 }
 
+// A page id as the choice holds it: an id that 32 bits do not hold is no page either way.
+__device__ __forceinline__ int32_t chosen_id(int64_t id) { return id < 0 || id > 0x7fffffff ? -1 : static_cast<int32_t>(id); }
+
 constexpr int kPickThreads = 512;
 
 // Sums of three counts over the CTA.  `phase` alternates two buffers, so one barrier is enough.
@@ -316,7 +322,7 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const PagedInt4
   int32_t* out = p.page_table + static_cast<int64_t>(row) * p.take;
   if (tid == 0) p.page_lens[row] = tokens - (count > p.take ? (count - p.take) * p.page_size : 0);
   if (count <= p.take) {
-    for (int n = tid; n < p.take; n += kPickThreads) out[n] = n < count ? static_cast<int32_t>(page_id(p, b, 0, n)) : -1;
+    for (int n = tid; n < p.take; n += kPickThreads) out[n] = n < count ? chosen_id(page_id(p, b, 0, n)) : -1;
     return;
   }
   const uint32_t* mine = keys + static_cast<int64_t>(row) * p.table_width;
@@ -379,14 +385,14 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const PagedInt4
   visit([&](int n, uint32_t key) {
     if (n >= end) return;
     if (key > least) {
-      out[before_above + min(before_equal, ties)] = static_cast<int32_t>(page_id(p, b, 0, n));
+      out[before_above + min(before_equal, ties)] = chosen_id(page_id(p, b, 0, n));
       ++before_above;
     } else if (key == least) {
-      if (before_equal < ties) out[before_above + before_equal] = static_cast<int32_t>(page_id(p, b, 0, n));
+      if (before_equal < ties) out[before_above + before_equal] = chosen_id(page_id(p, b, 0, n));
       ++before_equal;
     }
   });
-  if (tid == 0) out[p.take - 1] = static_cast<int32_t>(page_id(p, b, 0, count - 1));
+  if (tid == 0) out[p.take - 1] = chosen_id(page_id(p, b, 0, count - 1));
 }
 
 // Bytes of the keys, a multiple of 16.
@@ -455,7 +461,7 @@ int qf_int4_key_bounds(const qf_paged_int4_args* args, void* stream) {
   const int pages_each = static_cast<int>(spanned < p.table_width ? spanned : p.table_width);
   const int64_t units = static_cast<int64_t>(p.batch) * p.kv_heads * pages_each;
   QF_REQUIRE(units < (1LL << 31) - 4, "too many pages in one call");
-  const int tiles = p.page_size / kInt4Tile, warps_each = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1, pages_a_cta = kBoundWarps / warps_each;
+  const int tiles = p.page_size / kInt4Tile, warps_each = tiles >= kManyTiles ? kBoundWarps : 1, pages_a_cta = kBoundWarps / warps_each;
   const dim3 grid(static_cast<unsigned>((units + pages_a_cta - 1) / pages_a_cta));
   const Divisor by_each = make_divisor(pages_each);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -59,7 +59,7 @@ def test_magnitudes(package, cuda_device, dtype):
 
 
 def test_large_and_tiny_bf16(package, cuda_device):
-    for gain in (1e15, 1e-15):
+    for gain in (1e15, 1e-15, 1e33, 1e37):
         q, pool, table, lens = plain.make_cache([40, 200], dtype=torch.bfloat16, gain=gain, seed=2)
         _check(package, cuda_device, q, pool, table, lens)
     for query in (1e15, 1e-15):
@@ -222,6 +222,19 @@ def _decode_state(device, dtype=torch.float16, page=32, prompt=(200, 37, 90), st
 
 def _slots(table, b, positions, page):
     return table[b, positions // page].long() * page + positions % page
+
+
+def test_page_ids_beyond_32_bits_stay_outside_the_pool(package, cuda_device):
+    """An id of 2^32 + 5 must not come out of the choice as page 5."""
+    q, pool, table, lens = plain.make_cache([64, 300], seed=4)
+    k, _ = plain.rows(pool, q.dtype)
+    limits = plain.bounds(k, table, lens, q.dtype, 10 ** 6, torch.zeros(pool.shape[0], 2, 2, 128, dtype=q.dtype))
+    wide = table.long()
+    wide[0, 1], wide[1, 18] = 2 ** 32 + 5, 2 ** 33  # a page of a row whose pages are all taken, and a newest page
+    out, pages, held = package.sparse_decode_attention_int4(*(t.to(cuda_device) for t in (q, pool, limits, wide, lens)), num_pages=6)
+    assert package.cabi.device_status() == 2
+    assert pages[0, :, 1].tolist() == [-1, -1] and pages[1, :, 5].tolist() == [-1, -1]
+    plain.assert_attention(out, *plain.attention(q, *plain.rows(pool, q.dtype), pages.cpu(), held.cpu()))
 
 
 @pytest.mark.parametrize("captured", [False, True])
