@@ -85,13 +85,15 @@ __device__ __forceinline__ float max2_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// A warp takes a page, or four warps a page of kManyTiles and more; a lane holds eight channels of
+// A warp takes a page, or four warps a page of kManyTiles and more, or two or four where pages are few;
+// a lane holds eight channels of
 // 16 / (32 / (D / 8)) tokens of a tile, all loaded at once, and two tokens a step of the
 // three-operand minimum and maximum.  Rounding to T is monotone and comes once, after the warps of a
 // page have met.  Bound by issue, 25 instructions an eight codes: 16 prompts of 4096..8192 tokens
 // (2 x 128, pages of 64, 16 MB) take 10.7 us, a step's newest pages of 64 sequences 2.3 us.  Four warps
 // a page against one, the same prompts: pages of 64 tokens 14.8 and 10.7 us, of 128 12.0 and 15.5, of
-// 256 11.1 and 22.7.
+// 256 11.1 and 22.7; the newest page of each of 32 sequences ahead of their sparse attention, pages of
+// 64: 37.2 us in all and 40.0.
 constexpr int kBoundWarps = 4, kManyTiles = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kBoundWarps) key_bounds_kernel(const PagedInt4 p, const Divisor by_each, int warps_each) {
@@ -461,7 +463,10 @@ int qf_int4_key_bounds(const qf_paged_int4_args* args, void* stream) {
   const int pages_each = static_cast<int>(spanned < p.table_width ? spanned : p.table_width);
   const int64_t units = static_cast<int64_t>(p.batch) * p.kv_heads * pages_each;
   QF_REQUIRE(units < (1LL << 31) - 4, "too many pages in one call");
-  const int tiles = p.page_size / kInt4Tile, warps_each = tiles >= kManyTiles ? kBoundWarps : 1, pages_a_cta = kBoundWarps / warps_each;
+  const int tiles = p.page_size / kInt4Tile;
+  const bool few = units <= 4LL * sm_count();  // of them a warp each would leave schedulers idle
+  const int warps_each = tiles >= (few ? 4 : kManyTiles) ? 4 : tiles >= 2 && few ? 2 : 1;
+  const int pages_a_cta = kBoundWarps / warps_each;
   const dim3 grid(static_cast<unsigned>((units + pages_a_cta - 1) / pages_a_cta));
   const Divisor by_each = make_divisor(pages_each);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
