@@ -108,9 +108,16 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// What a call shares out: units of all rows (fewer than 2^31), units of a CTA.
+// A row costs its units and one more: its queries' way to the registers and its result's way out
+// take about as long as a unit.  A place in a row counts that one first, so unit u is at place u + 1.
+// Shares are runs of places: without the extra one the CTAs with the most short rows of 256 sequences of
+// 64..4096 tokens ended at 50 us and half of them before 42.5.
+__device__ __forceinline__ int row_units(int tokens) { return (tokens + kUnit - 1) / kUnit; }
+__device__ __forceinline__ int row_places(int tokens) { return tokens > 0 ? row_units(tokens) + 1 : 0; }
+
+// What a call shares out: places of all rows (fewer than 2^31), places of a CTA.
 struct Plan {
-  int units;
+  int places;
   int share;
 };
 
@@ -119,7 +126,7 @@ __device__ __forceinline__ int row_tokens_at(const PagedInt4& p, int row) {
   return static_cast<int>(row_tokens(p, at.x, at.y));
 }
 
-// Shared by a CTA's warps: prefix sums of the rows' units, thread by thread (`chunk` rows each),
+// Shared by a CTA's warps: prefix sums of the rows' places, thread by thread (`chunk` rows each),
 // and the lengths of the first rows.
 constexpr int kRowsKept = 2048;
 template <int kWarps>
@@ -136,7 +143,7 @@ __device__ __forceinline__ Plan make_plan(const PagedInt4& p, Shares<kWarps>& s,
   int mine = 0;
   for (int r = first; r < first + chunk && r < rows; ++r) {
     const int tokens = row_tokens_at(p, r);
-    mine += (tokens + kUnit - 1) / kUnit;
+    mine += row_places(tokens);
     if (r < kRowsKept) s.tokens[r] = tokens;
   }
   int sum = mine;
@@ -149,13 +156,13 @@ __device__ __forceinline__ Plan make_plan(const PagedInt4& p, Shares<kWarps>& s,
   s.prefix[threadIdx.x] = sum - mine;  // within the warp's rows
   __syncthreads();
   Plan plan;
-  plan.units = __reduce_add_sync(0xffffffffu, lane < kWarps ? s.warp[lane] : 0);
-  plan.share = (plan.units + ctas - 1) / ctas;
-  if (plan.share < kWarps) plan.share = kWarps;  // a unit a warp at least: fewer pieces for the second kernel
+  plan.places = __reduce_add_sync(0xffffffffu, lane < kWarps ? s.warp[lane] : 0);
+  plan.share = (plan.places + ctas - 1) / ctas;
+  if (plan.share < kWarps) plan.share = kWarps;  // a place a warp at least: fewer pieces for the second kernel
   return plan;
 }
 
-// The thread whose rows hold unit `first`, and the units before those rows.
+// The thread whose rows hold place `first`, and the places before those rows.
 template <int kWarps>
 __device__ __forceinline__ int2 find_rows(const Shares<kWarps>& s, int first, int lane) {
   const int mine = lane < kWarps ? s.warp[lane] : 0;
@@ -177,23 +184,25 @@ __device__ __forceinline__ int tokens_of(const PagedInt4& p, const Shares<kWarps
   return row < kRowsKept ? s.tokens[row] : row_tokens_at(p, row);
 }
 
-// The next 32 units to request: lane i holds the two tiles of unit i, kNoTile for one behind the
-// row's end or in a page outside the pool.
+// The next units to request, 32 or fewer: lane i holds the two tiles of unit i, kNoTile for one
+// behind the row's end or in a page outside the pool.
 struct Requests {
-  int row, unit;  // the next one
-  int left;
+  int row, place;  // the next one
+  int left;        // places
+  int count, next; // units held, and the first of them not requested yet
   uint32_t tile[2];
 
   template <int kWarps>
   __device__ __forceinline__ void refill(const PagedInt4& p, const Shares<kWarps>& s, int lane) {
-    int filled = 0, mine = -1, mine_row = 0, mine_tokens = 0;
-    while (filled < 32 && left > 0 && row < p.batch * p.kv_heads) {
-      const int tokens = tokens_of(p, s, row);
-      const int units = (tokens + kUnit - 1) / kUnit;
-      const int n = min(min(32 - filled, units - unit), left);
-      if (lane >= filled && lane < filled + n) mine = unit + lane - filled, mine_row = row, mine_tokens = tokens;
-      filled += n, left -= n, unit += n;
-      if (unit >= units) ++row, unit = 0;
+    int mine = -1, mine_row = 0, mine_tokens = 0;
+    count = next = 0;
+    while (count < 32 && left > 0 && row < p.batch * p.kv_heads) {
+      const int tokens = tokens_of(p, s, row), places = row_places(tokens);
+      if (place == 0 && places > 0) place = 1, --left;
+      const int n = min(min(32 - count, places - place), left);
+      if (lane >= count && lane < count + n) mine = place - 1 + lane - count, mine_row = row, mine_tokens = tokens;
+      count += n, left -= n, place += n;
+      if (place >= places) ++row, place = 0;
     }
     tile[0] = tile[1] = kNoTile;
     if (mine < 0) return;
@@ -686,44 +695,44 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
   if (!p.early) dependency_wait();
   const Plan plan = make_plan(p, s_shares, chunk, ctas);
 
-  // this warp's units
-  const int cta_first = static_cast<int>(min(static_cast<int64_t>(plan.share) * cta, static_cast<int64_t>(plan.units)));
-  const int cta_units = min(plan.share, plan.units - cta_first);
-  const int first = cta_first + static_cast<int>(static_cast<int64_t>(cta_units) * warp / kWarps);
-  const int units = cta_first + static_cast<int>(static_cast<int64_t>(cta_units) * (warp + 1) / kWarps) - first;
+  // this warp's places
+  const int cta_first = static_cast<int>(min(static_cast<int64_t>(plan.share) * cta, static_cast<int64_t>(plan.places)));
+  const int cta_places = min(plan.share, plan.places - cta_first);
+  const int first = cta_first + static_cast<int>(static_cast<int64_t>(cta_places) * warp / kWarps);
+  const int end = cta_first + static_cast<int>(static_cast<int64_t>(cta_places) * (warp + 1) / kWarps);
 
   Requests ahead{};
-  if (units > 0) {
+  if (first < end) {
     const int2 found = find_rows(s_shares, first, lane);
     int before = first - found.y;
     for (ahead.row = found.x * chunk; ahead.row < p.batch * p.kv_heads; ++ahead.row) {
-      const int in_row = (tokens_of(p, s_shares, ahead.row) + kUnit - 1) / kUnit;
-      if (before < in_row) break;
-      before -= in_row;
+      const int places = row_places(tokens_of(p, s_shares, ahead.row));
+      if (before < places) break;
+      before -= places;
     }
-    ahead.unit = before;
-    ahead.left = units;
+    ahead.place = before;
+    ahead.left = end - first;
   }
-  int id = ahead.row, in_row = ahead.unit;  // of the unit at hand
-  if (units > 0) ahead.refill(p, s_shares, lane);
+  int id = ahead.row, place = ahead.place;  // of the unit at hand
+  if (first < end) ahead.refill(p, s_shares, lane);
   if (p.early) dependency_wait();
 
-  if (units > 0) {
+  if (ahead.count > 0) {  // a unit, not the first place of a row alone
     Row<T, D, NT> row;
     uint4 queries[NT][D / kInt4Group];
-    row.load(p, id, group, lane, queries);
+    bool loaded = place > 0 || row_places(tokens_of(p, s_shares, id)) > 0;  // else a row without tokens stands here
+    if (loaded) row.load(p, id, group, lane, queries);
 
-    int wanted = 0;                                     // units requested
     uint32_t request_at = smem_u32(ring) + 16 * lane;  // where this lane's part of the next goes
     const uint32_t ring_end = request_at + S::kRing;
     const uint8_t* pool = p.pool + 16 * lane;
     // One group of copies a call, an empty one behind the last unit.
     auto request = [&]() {
-      if (wanted < units) {
-        if ((wanted & 31) == 0 && wanted > 0) ahead.refill(p, s_shares, lane);
+      if (ahead.next == ahead.count && ahead.left > 0) ahead.refill(p, s_shares, lane);
+      if (ahead.next < ahead.count) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const uint32_t tile = __shfl_sync(0xffffffffu, ahead.tile[k], wanted & 31);
+          const uint32_t tile = __shfl_sync(0xffffffffu, ahead.tile[k], ahead.next);
           const bool real = tile != kNoTile;
           const uint8_t* src = pool + (real ? static_cast<int64_t>(tile) * S::kTileBytes : 0);
 #pragma unroll
@@ -733,7 +742,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
             copy16(request_at + k * S::kTileBytes + kDone, src + kDone, real);
           }
         }
-        ++wanted;
+        ++ahead.next;
         request_at = request_at + S::kStageBytes == ring_end ? request_at + S::kStageBytes - S::kRing : request_at + S::kStageBytes;
       }
       copies_close();
@@ -741,23 +750,27 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
 #pragma unroll
     for (int k = 0; k < S::kStages - 1; ++k) request();
 
-    int done = 0;
+    int now = first;  // place, of all rows
     const uint8_t* at = ring;
-    while (done < units) {
+    while (now < end) {
       int tokens = 0;
-      for (; id < p.batch * p.kv_heads; ++id, in_row = 0) {
+      for (; id < p.batch * p.kv_heads; ++id, place = 0, loaded = false) {
         tokens = tokens_of(p, s_shares, id);
-        if (in_row * kUnit < tokens) break;
+        if (place < row_places(tokens)) break;
       }
       if (id >= p.batch * p.kv_heads) break;  // lengths that change under a call must not lead it out of the batch
-      const int in_all = (tokens + kUnit - 1) / kUnit;
-      const int n = min(in_all - in_row, units - done);
-      if (done > 0) row.load(p, id, group, lane, queries);
+      if (place == 0) {
+        place = 1;
+        if (++now == end) break;
+      }
+      const int in_all = row_units(tokens), in_row = place - 1;
+      const int n = min(in_all - in_row, end - now);
+      if (!loaded) row.load(p, id, group, lane, queries);
       row.start(p, queries, lane);
       const bool starts = in_row == 0, ends = in_row + n >= in_all;
       if (starts && lane == 0) {
-        const int beyond = first + done + in_all - cta_first;  // units of the row's end from this CTA's first on
-        if (beyond > cta_units) s_shared_row = make_int2(id, cta + (beyond - 1) / plan.share);
+        const int beyond = now + in_all - cta_first;  // places of the row's end from this CTA's first on
+        if (beyond > cta_places) s_shared_row = make_int2(id, cta + (beyond - 1) / plan.share);
       }
       int left = tokens - in_row * kUnit;
       for (int k = 0; k < n; ++k, left -= kUnit) {
@@ -767,12 +780,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
         row.unit(at, left, lane);
         at = at + S::kStageBytes == ring + S::kRing ? ring : at + S::kStageBytes;
       }
-      done += n;
+      now += n, place += n;
       row.finish(lane);
       if (starts && ends) {
         row.write_out(p, id, group, lane);
       } else {
-        const bool last = done == units;
+        const bool last = end - now <= 1;  // one more place is the next row's first
         __syncwarp();
         row.deposit(last ? reinterpret_cast<float*>(ring) : scratch.warp_pieces + static_cast<int64_t>(cta * kWarps + warp) * S::kPiece, lane);
         if (lane == 0) {
@@ -780,7 +793,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
           s_flags[2 * warp + (last ? 1 : 0)] = (starts ? kRowStart : 0) | (ends ? kRowEnd : 0);
         }
       }
-      in_row += n;
+      loaded = false;
     }
     copies_wait<0>();
   }
