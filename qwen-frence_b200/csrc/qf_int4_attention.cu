@@ -28,10 +28,11 @@
 // of them the masks and shifts that take codes apart, on four schedulers of which each is busy six
 // cycles in ten.  With all tiles in one page, that is with no memory to wait for, calls take 7 % less
 // time, so issue and dependences bound it, and for short calls the way to the first tile (lengths, table,
-// tile: 3 us) and the two launches.  64 sequences of 129..4097 tokens, 12 heads on 2 of 128: 20 us, 42 MB,
-// 2.1 TB/s; 256 of 64..4096, 16 on 4 of 64: 49 us, 172 MB, 3.5 TB/s; one of 513: 7.7 us.
-// Warps an SM, D = 128: 8 take 22 us for the first, 10 22.3, 12 20.0, 14 20.9, 16 21.2 (from 13 on the
-// registers no longer hold a row: 168 against 128 a thread); D = 64: 12 take 54 us, 16 52, 20 54.
+// tile: 3 us) and the two launches.  64 sequences of 129..4097 tokens, 12 heads on 2 of 128: 19.4 us, 42 MB,
+// 2.2 TB/s; 256 of 64..4096, 16 on 4 of 64: 48 us, 172 MB, 3.6 TB/s; one of 513: 7.9 us (both kernels, in
+// graphs).  Warps an SM, measured before rows counted a place of their own, D = 128: 8 take 22 us for the
+// first, 10 22.3, 12 20.0, 14 20.9, 16 21.2 (from 13 on the registers no longer hold a row: 168 against 128 a
+// thread); D = 64: 12 take 54 us, 16 52, 20 54.
 // Taking the next unit's scores beside this one's values gives the schedulers two chains to choose from
 // and cost 3 to 5 %; V words rotated so that no two lanes meet in a bank changed nothing.
 #include <algorithm>
@@ -861,7 +862,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
 }
 
 // Rows that span CTAs: one CTA a CTA of the first kernel, for the row that starts there and goes on,
-// `each` warps a query head, the pieces dealt out to those in turn.
+// `each` warps a query head, the pieces dealt out to those in turn.  Bound by latency: two dependent
+// loads and a barrier; about 2 us, most of it the launch.  With 32 registers a thread, so that a CTA
+// could stand by beside the first kernel's, its loads are no longer in flight together: 3 us more.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(1024) int4_combine_kernel(const PagedInt4 p, int ctas, int each) {
   using S = Shape<D, NT>;
