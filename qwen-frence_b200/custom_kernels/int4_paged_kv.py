@@ -38,6 +38,7 @@ import torch
 
 TILE_TOKENS = 16
 MAX_GROUP = 16
+MAX_ITEMS = 2 ** 31 - 128  # threads of one write
 
 def _load_cabi():
     """The ctypes binding, loaded by path so this file works under any module name."""
@@ -247,8 +248,11 @@ def quantize_kv_pool_int4(k_pool, v_pool):
     _require(k_pool.is_cuda and v_pool.device == k_pool.device, "K/V pools must share one CUDA device")
     pool = empty_kv_pool_int4(pages, kv_heads, dim, page_size=page_size, device=k_pool.device)
     _require(v_pool.dtype == k_pool.dtype, "K/V pools must share FP16 or BF16 dtype")
-    _write(pool, (pages, kv_heads, dim, page_size), (0, k_pool.data_ptr(), v_pool.data_ptr(), 0),
-           (kv_heads * dim, dim, 1) * 4, k_pool, None, None, rows=pages * page_size, q_heads=0, base=1.0, rope_table=None)
+    step = max(1, MAX_ITEMS // (2 * kv_heads * (dim // 16) * page_size))  # pages a call has room for
+    for first in range(0, pages, step):
+        k, v, part = k_pool[first:first + step], v_pool[first:first + step], pool[first:first + step]
+        _write(part, (part.shape[0], kv_heads, dim, page_size), (0, k.data_ptr(), v.data_ptr(), 0), (kv_heads * dim, dim, 1) * 4,
+               k, None, None, rows=part.shape[0] * page_size, q_heads=0, base=1.0, rope_table=None)
     return pool
 
 
