@@ -3,6 +3,8 @@ codec's, whatever the layout of the inputs."""
 
 from __future__ import annotations
 
+from unittest import mock
+
 import pytest
 import torch
 
@@ -117,6 +119,16 @@ def test_codes_of_quotients_between_two(package, cuda_device, dtype):
     plain.store_fast(pool, torch.arange(rows), k, v)
     got = package.quantize_kv_pool_int4(*(t.to(cuda_device).view(rows // 16, 16, heads, dim) for t in (k, v)))
     _same_cache(got.cpu(), pool, dtype)
+
+
+def test_converting_pools_in_parts(package, cuda_device):
+    """Pools of more threads than one write takes are converted page range by page range: the same bytes."""
+    g = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(7, 32, 2, 128, generator=g).half().to(cuda_device) for _ in range(2))
+    whole = package.quantize_kv_pool_int4(k, v)
+    with mock.patch.object(package.kernel_module("int4_paged_kv"), "MAX_ITEMS", 3 * 32 * 32 + 5):
+        parts = package.quantize_kv_pool_int4(k, v)
+    assert torch.equal(whole, parts)
 
 
 def test_valid_tokens_empty_calls_and_positions_past_the_table(package, cuda_device):
