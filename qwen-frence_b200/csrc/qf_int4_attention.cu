@@ -692,7 +692,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
   uint8_t* ring = s_ring + warp * S::kRing;
   if (threadIdx.x < 2 * kWarps) s_row[threadIdx.x] = -1;
   if (threadIdx.x == 0) s_shared_row = make_int2(-1, -1);
-  release_dependents();
   if (!p.early) dependency_wait();
   const Plan plan = make_plan(p, s_shares, chunk, ctas);
 
@@ -800,6 +799,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
   }
   __syncthreads();
 
+  // Only now: CTAs of the kernel behind, standing by from the start, cost 1 to 4 % of a long call.
+  release_dependents();
   if (threadIdx.x == 0) scratch.shared_rows[cta] = s_shared_row;
   // rows without tokens
   for (int r = cta; r < p.batch * p.kv_heads; r += ctas) {
