@@ -200,7 +200,6 @@ template <typename T, int D>
 __global__ void __launch_bounds__(128) page_score_kernel(const PagedInt4 p, uint32_t* keys) {
   constexpr int kLanes = D / 8, kPages = 32 / kLanes, kMaxGroup = 16, kCtaPages = 4 * 2 * kPages;
   __shared__ __align__(16) float4 s_q[kMaxGroup][4][kLanes];  // two channels of a lane: neighbouring lanes, neighbouring banks
-  // No early release: the choice's CTAs, standing by, cost this kernel 2 to 4 us.
   if (!p.early) dependency_wait();
   const int row = blockIdx.y;
   const int2 at = row_place(p, row);
@@ -251,6 +250,7 @@ __global__ void __launch_bounds__(128) page_score_kernel(const PagedInt4 p, uint
     }
   }
   __syncthreads();
+  release_dependents();  // not from the start: kernels standing by cost this one 2 to 4 us, and to release at the end 1 us in front of one sequence
   for (; first < count - 1; first += step) {
     uint64_t low[8], high[8];
 #pragma unroll
@@ -295,82 +295,114 @@ __device__ __forceinline__ int32_t chosen_id(int64_t id) { return id < 0 || id >
 
 constexpr int kPickThreads = 512;
 
-// Sums of three counts over the CTA.  `phase` alternates two buffers, so one barrier is enough.
-__device__ __forceinline__ int3 cta_sums(int a, int b, int c, int (*s_sum)[3][kPickThreads / 32], int phase) {
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  a = __reduce_add_sync(0xffffffffu, a), b = __reduce_add_sync(0xffffffffu, b), c = __reduce_add_sync(0xffffffffu, c);
-  if (lane == 0) s_sum[phase][0][warp] = a, s_sum[phase][1][warp] = b, s_sum[phase][2][warp] = c;
-  __syncthreads();
-  const bool on = lane < kPickThreads / 32;
-  a = on ? s_sum[phase][0][lane] : 0, b = on ? s_sum[phase][1][lane] : 0, c = on ? s_sum[phase][2][lane] : 0;
-  return make_int3(__reduce_add_sync(0xffffffffu, a), __reduce_add_sync(0xffffffffu, b), __reduce_add_sync(0xffffffffu, c));
-}
-
-// One CTA a row.  The take - 1 largest keys of the pages before the newest: the smallest of them
-// two bits at a time, by counting the keys at or above three candidates (equal keys cost what
-// different ones do), then the pages in order, those that tie with it as long as there is room.
-// A thread holds a run of kHeld neighbouring keys in registers; longer rows are read again from
-// the second level cache every time.  Bound by the latency of its dozen or so rounds of counts: 2048
-// pages of one sequence take 6 us, with 16 keys a thread where 5 hold them 14.  (A histogram of digits
-// in shared memory with its bins summed by one thread took 25.)
+// One CTA a row.  The take - 1 largest keys of the pages before the newest: the smallest of them eight
+// bits at a time from the highest bit in which keys differ, by counting the keys that agree so far over
+// their next bits; it ends with a bin that is taken whole, mostly the second.  Then the pages in order,
+// those that tie with the smallest as long as there is room.  A thread holds a run of kHeld neighbouring
+// keys and their pages in registers; longer rows are read again from the second level cache every time.
+// Bound by latency, loads and barriers: 2048 pages of one sequence take 6.7 us by themselves with the
+// launch; two bits at a time, counted in registers, took 10.6.
 template <int kHeld>
 __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const PagedInt4 p, const uint32_t* keys) {
-  __shared__ int s_sum[2][3][kPickThreads / 32];
+  constexpr int kBins = 256, kPasses = 4;
+  __shared__ __align__(16) int s_bins[kPasses][kBins];
+  __shared__ uint32_t s_low[kPickThreads / 32], s_high[kPickThreads / 32];
   __shared__ int2 s_scan[kPickThreads / 32];
   release_dependents();
-  dependency_wait();
   const int row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  for (int i = tid; i < kPasses * kBins; i += kPickThreads) (&s_bins[0][0])[i] = 0;
+  if (!p.early) dependency_wait();
   const int2 at = row_place(p, row);
   const int b = at.x;
-  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int tokens = static_cast<int>(row_tokens(p, b, 0));
   const int count = quotient(tokens + p.page_size - 1, p.by_page);
   int32_t* out = p.page_table + static_cast<int64_t>(row) * p.take;
-  if (tid == 0) p.page_lens[row] = tokens - (count > p.take ? (count - p.take) * p.page_size : 0);
-  if (count <= p.take) {
+  const int others = count - 1, want = p.take - 1;
+  const int run = kHeld > 0 ? kHeld : (others + kPickThreads - 1) / kPickThreads;
+  const int first = min(tid * run, others), end = min(first + run, others);
+  const bool all = count <= p.take;
+  uint32_t held[kHeld > 0 ? kHeld : 1];
+  int32_t pages[kHeld > 0 ? kHeld : 1];
+  if constexpr (kHeld > 0) {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) pages[k] = !all && first + k < end ? chosen_id(page_id(p, b, 0, first + k)) : -1;
+  }
+  if (p.early) dependency_wait();
+  if (tid == 0) p.page_lens[row] = tokens - (all ? 0 : (count - p.take) * p.page_size);
+  if (all) {
     for (int n = tid; n < p.take; n += kPickThreads) out[n] = n < count ? chosen_id(page_id(p, b, 0, n)) : -1;
     return;
   }
   const uint32_t* mine = keys + static_cast<int64_t>(row) * p.table_width;
-  const int others = count - 1, want = p.take - 1;
-  const int run = kHeld > 0 ? kHeld : (others + kPickThreads - 1) / kPickThreads;
-  const int first = min(tid * run, others), end = min(first + run, others);
-  uint32_t held[kHeld > 0 ? kHeld : 1];
   if constexpr (kHeld > 0) {
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) held[k] = first + k < end ? mine[first + k] : 0u;
   }
-  // `visit` sees this thread's keys; places behind the last count as key 0, below every candidate
+  // `visit` sees this thread's keys, those of places behind the last too
   auto visit = [&](auto&& f) {
     if constexpr (kHeld > 0) {
 #pragma unroll
-      for (int k = 0; k < kHeld; ++k) f(first + k, held[k]);
+      for (int k = 0; k < kHeld; ++k) f(first + k, held[k], pages[k]);
     } else {
-      for (int n = first; n < end; ++n) f(n, mine[n]);
+      for (int n = first; n < end; ++n) f(n, mine[n], -1);
     }
   };
-  // the largest value that at least `want` keys reach; the bits that all keys share are known
+  auto id_of = [&](int n, int32_t page) { return kHeld > 0 ? page : chosen_id(page_id(p, b, 0, n)); };
+  // the bits that all keys share
   uint32_t low = 0xffffffffu, high = 0u;
-  visit([&](int n, uint32_t key) {
+  visit([&](int n, uint32_t key, int32_t) {
     if (n < end) low = min(low, key), high = max(high, key);
   });
   low = __reduce_min_sync(0xffffffffu, low), high = __reduce_max_sync(0xffffffffu, high);
-  if (lane == 0) s_sum[1][0][warp] = static_cast<int>(low), s_sum[1][1][warp] = static_cast<int>(high);
+  if (lane == 0) s_low[warp] = low, s_high[warp] = high;
   __syncthreads();
-  low = __reduce_min_sync(0xffffffffu, lane < kPickThreads / 32 ? static_cast<uint32_t>(s_sum[1][0][lane]) : 0xffffffffu);
-  high = __reduce_max_sync(0xffffffffu, lane < kPickThreads / 32 ? static_cast<uint32_t>(s_sum[1][1][lane]) : 0u);
-  const int top = low == high ? -1 : (31 - __clz(low ^ high)) & ~1;  // lowest bit of the first pair that differs
-  uint32_t least = top < 0 ? low : top >= 30 ? 0u : high >> (top + 2) << (top + 2);
-  int phase = 0;
-  for (int shift = top; shift >= 0; shift -= 2, phase ^= 1) {
-    const uint32_t one = least | (1u << shift), two = least | (2u << shift), three = least | (3u << shift);
-    int a = 0, c = 0, e = 0;
-    visit([&](int, uint32_t key) { a += key >= one, c += key >= two, e += key >= three; });
-    const int3 reached = cta_sums(a, c, e, s_sum, phase);
-    least = reached.z >= want ? three : reached.y >= want ? two : reached.x >= want ? one : least;
+  low = __reduce_min_sync(0xffffffffu, lane < kPickThreads / 32 ? s_low[lane] : 0xffffffffu);
+  high = __reduce_max_sync(0xffffffffu, lane < kPickThreads / 32 ? s_high[lane] : 0u);
+  // `least`: the largest value that at least `want` keys reach, its bits from `shift` on so far
+  uint32_t least = low;
+  if (low != high) {
+    int shift = max(24 - __clz(low ^ high), 0), left = want;
+    uint32_t bins = kBins;  // of the pass: keys that agree so far are less than so many steps off
+    least = shift == 24 ? 0u : high >> (shift + 8) << (shift + 8);
+    for (int pass = 0;; ++pass) {
+      visit([&](int n, uint32_t key, int32_t) {
+        const uint32_t bin = (key ^ least) >> shift;
+        if (n < end && bin < bins) atomicAdd(&s_bins[pass][bin], 1);
+      });
+      __syncthreads();
+      // every warp for itself: eight bins a lane, the lanes' sums from the top, and the bin in which the
+      // count passes `left`
+      const int4 x = reinterpret_cast<const int4*>(s_bins[pass])[2 * lane], y = reinterpret_cast<const int4*>(s_bins[pass])[2 * lane + 1];
+      const int n8[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      const int mine8 = (x.x + x.y) + (x.z + x.w) + ((y.x + y.y) + (y.z + y.w));
+      int from = mine8;  // of this lane and those above
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int z = __shfl_down_sync(0xffffffffu, from, off);
+        if (lane + off < 32) from += z;
+      }
+      int over = from - mine8, bin = 0, size = 0;  // keys in the bins above, the bin, its keys
+      bool found = false;
+#pragma unroll
+      for (int k = 7; k >= 0; --k) {
+        if (!found) {
+          bin = 8 * lane + k, size = n8[k];
+          found = over + size >= left;
+          if (!found) over += size;
+        }
+      }
+      const int lane_of = 31 - __clz(__ballot_sync(0xffffffffu, from >= left));  // the highest such lane holds the bin
+      over = __shfl_sync(0xffffffffu, over, lane_of), bin = __shfl_sync(0xffffffffu, bin, lane_of), size = __shfl_sync(0xffffffffu, size, lane_of);
+      least |= static_cast<uint32_t>(bin) << shift;
+      left -= over;
+      if (size == left || shift == 0) break;
+      bins = min(1u << shift, static_cast<uint32_t>(kBins));
+      shift = max(shift - 8, 0);
+    }
   }
   int above = 0, equal = 0;
-  visit([&](int n, uint32_t key) { above += n < end && key > least, equal += n < end && key == least; });
+  visit([&](int n, uint32_t key, int32_t) { above += n < end && key > least, equal += n < end && key == least; });
   // exclusive sums of both over the threads before this one
   int2 sum = make_int2(above, equal);
 #pragma unroll
@@ -388,13 +420,13 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const PagedInt4
     all_above += x.x;
   }
   const int ties = want - all_above;  // the first so many of the keys equal to `least`
-  visit([&](int n, uint32_t key) {
+  visit([&](int n, uint32_t key, int32_t page) {
     if (n >= end) return;
     if (key > least) {
-      out[before_above + min(before_equal, ties)] = chosen_id(page_id(p, b, 0, n));
+      out[before_above + min(before_equal, ties)] = id_of(n, page);
       ++before_above;
     } else if (key == least) {
-      if (before_equal < ties) out[before_above + before_equal] = chosen_id(page_id(p, b, 0, n));
+      if (before_equal < ties) out[before_above + before_equal] = id_of(n, page);
       ++before_equal;
     }
   });
