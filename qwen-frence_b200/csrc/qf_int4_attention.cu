@@ -20,17 +20,19 @@
 // a barrier a stage, the same ring took 125 instructions more a unit and 7 % more time at D = 64); warps
 // share nothing until their units are done.  A row that one warp holds whole is written from its
 // registers; what the warps of a CTA hold of one row is summed at the CTA's end, and rows that span
-// CTAs by a second kernel, in the order of the tiles: the same call gives the same bits.  Table and
-// lengths are read while the kernel in front drains, unless it writes them.
+// CTAs by a second kernel, in the order of the tiles: the same call gives the same bits.  Where tables
+// are so short that it ends sooner, a row is one CTA's alone or one cluster's, whose CTAs join their sums
+// behind a barrier, without a second kernel (row_parts).  Table and lengths are read while the kernel in
+// front drains, unless it writes them.
 //
 // Bound.  The cache's 5 bits a channel come in at the memory's rate only if the SM spends no more than
 // 110 cycles on a tile of D = 128 (55 at D = 64); it issues about 250 (200) instructions a tile, a third
 // of them the masks and shifts that take codes apart, on four schedulers of which each is busy six
 // cycles in ten.  With all tiles in one page, that is with no memory to wait for, calls take 7 % less
 // time, so issue and dependences bound it, and for short calls the way to the first tile (lengths, table,
-// tile: 3 us) and the two launches.  64 sequences of 129..4097 tokens, 12 heads on 2 of 128: 19.4 us, 42 MB,
-// 2.2 TB/s; 256 of 64..4096, 16 on 4 of 64: 48 us, 172 MB, 3.6 TB/s; one of 513: 7.9 us (both kernels, in
-// graphs).  Warps an SM, measured before rows counted a place of their own, D = 128: 8 take 22 us for the
+// tile: 3 us) and the launches.  64 sequences of 129..4097 tokens, 12 heads on 2 of 128: 18.4 us, 42 MB,
+// 2.3 TB/s; 256 of 64..4096, 16 on 4 of 64: 45.8 us, 172 MB, 3.8 TB/s; one of 513: 6.9 us (all in graphs).
+//  Warps an SM, measured before rows counted a place of their own, D = 128: 8 take 22 us for the
 // first, 10 22.3, 12 20.0, 14 20.9, 16 21.2 (from 13 on the registers no longer hold a row: 168 against 128 a
 // thread); D = 64: 12 take 54 us, 16 52, 20 54.
 // Taking the next unit's scores beside this one's values gives the schedulers two chains to choose from
@@ -121,6 +123,9 @@ struct Plan {
   int places;
   int share;
 };
+
+// First unit of CTA `rank` of the `parts` that a row is split over.
+__device__ __forceinline__ int part_first(int units, int rank, int parts) { return static_cast<int>(static_cast<uint32_t>(units) * rank / parts); }
 
 __device__ __forceinline__ int row_tokens_at(const PagedInt4& p, int row) {
   const int2 at = row_place(p, row);
@@ -652,6 +657,33 @@ struct Merge {
   }
 };
 
+// The weighted sum of the pieces of `chain`, whose lanes hold the weights; at(k): piece k's channels of this lane.
+template <int D, typename At>
+__device__ __forceinline__ Merge<D> merged(unsigned chain, float weight, At at) {
+  Merge<D> merge;
+  merge.clear();
+  const int i = __ffs(chain) - 1;
+  for (unsigned left = chain; left != 0u;) {
+    float x[4][Merge<D>::C], scale[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {  // four pieces in flight; the first one again, weightless, where fewer are left
+      const int k = left != 0u ? __ffs(left) - 1 : i;
+      scale[n] = __shfl_sync(0xffffffffu, weight, k);
+      if (left == 0u) scale[n] = 0.f;
+      left &= left - 1;
+      Merge<D>::load(at(k), x[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) merge.add(x[n], scale[n]);
+  }
+  return merge;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
@@ -676,7 +708,7 @@ __host__ __device__ Scratch carve(void* workspace, int ctas) {
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kernel(const PagedInt4 p, int chunk) {
+__global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kernel(const PagedInt4 p, int chunk, int parts) {
   using S = Shape<D, NT>;
   constexpr int kWarps = S::kWarps;
   extern __shared__ __align__(128) uint8_t s_ring[];
@@ -693,22 +725,36 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
   if (threadIdx.x < 2 * kWarps) s_row[threadIdx.x] = -1;
   if (threadIdx.x == 0) s_shared_row = make_int2(-1, -1);
   if (!p.early) dependency_wait();
-  const Plan plan = make_plan(p, s_shares, chunk, ctas);
-
-  // this warp's places
-  const int cta_first = static_cast<int>(min(static_cast<int64_t>(plan.share) * cta, static_cast<int64_t>(plan.places)));
-  const int cta_places = min(plan.share, plan.places - cta_first);
-  const int first = cta_first + static_cast<int>(static_cast<int64_t>(cta_places) * warp / kWarps);
-  const int end = cta_first + static_cast<int>(static_cast<int64_t>(cta_places) * (warp + 1) / kWarps);
-
+  // this warp's places, of all rows or (parts > 0) of this cluster's row
+  Plan plan;
+  int cta_first, cta_places, first, end, units = 0;
+  const int rank = parts > 0 ? cta % parts : 0;
   Requests ahead{};
+  if (parts > 0) {
+    ahead.row = cta / parts;
+    const int tokens = row_tokens_at(p, ahead.row);
+    if (threadIdx.x == 0) s_shares.tokens[ahead.row] = tokens;
+    __syncthreads();
+    units = row_units(tokens);
+    plan.places = units + 1, plan.share = units + 1;
+    cta_first = 1 + part_first(units, rank, parts), cta_places = 1 + part_first(units, rank + 1, parts) - cta_first;
+  } else {
+    plan = make_plan(p, s_shares, chunk, ctas);
+    cta_first = static_cast<int>(min(static_cast<int64_t>(plan.share) * cta, static_cast<int64_t>(plan.places)));
+    cta_places = min(plan.share, plan.places - cta_first);
+  }
+  first = cta_first + static_cast<int>(static_cast<int64_t>(cta_places) * warp / kWarps);
+  end = cta_first + static_cast<int>(static_cast<int64_t>(cta_places) * (warp + 1) / kWarps);
   if (first < end) {
-    const int2 found = find_rows(s_shares, first, lane);
-    int before = first - found.y;
-    for (ahead.row = found.x * chunk; ahead.row < p.batch * p.kv_heads; ++ahead.row) {
-      const int places = row_places(tokens_of(p, s_shares, ahead.row));
-      if (before < places) break;
-      before -= places;
+    int before = first;
+    if (parts == 0) {
+      const int2 found = find_rows(s_shares, first, lane);
+      before -= found.y;
+      for (ahead.row = found.x * chunk; ahead.row < p.batch * p.kv_heads; ++ahead.row) {
+        const int places = row_places(tokens_of(p, s_shares, ahead.row));
+        if (before < places) break;
+        before -= places;
+      }
     }
     ahead.place = before;
     ahead.left = end - first;
@@ -801,9 +847,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
 
   // Only now: CTAs of the kernel behind, standing by from the start, cost 1 to 4 % of a long call.
   release_dependents();
-  if (threadIdx.x == 0) scratch.shared_rows[cta] = s_shared_row;
+  if (threadIdx.x == 0 && parts == 0) scratch.shared_rows[cta] = s_shared_row;
   // rows without tokens
-  for (int r = cta; r < p.batch * p.kv_heads; r += ctas) {
+  for (int r = parts == 0 ? cta : rank == 0 ? cta / parts : p.batch * p.kv_heads; r < p.batch * p.kv_heads; r += ctas) {
     if (tokens_of(p, s_shares, r) != 0) continue;
     const int2 at = row_place(p, r);
     for (int i = threadIdx.x; i < group * (D / 8); i += S::kThreads) {
@@ -833,23 +879,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
     for (; head < group; head += kWarps) {
       float2 ml = make_float2(-INFINITY, 0.f);
       if (my_row == id) ml = *reinterpret_cast<const float2*>(piece_of(lane) + S::kHeads * S::kStride + 2 * head);
-      Merge<D> merge;
-      merge.clear();
       const float top = warp_max(ml.x);
       const float weight = my_row == id ? fast_exp2(ml.x - top) : 0.f;
-      for (unsigned left = chain; left != 0u;) {
-        float x[4][Merge<D>::C], scale[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {  // four pieces in flight; the first one again, weightless, where fewer are left
-          const int k = left != 0u ? __ffs(left) - 1 : i;
-          scale[n] = __shfl_sync(0xffffffffu, weight, k);
-          if (left == 0u) scale[n] = 0.f;
-          left &= left - 1;
-          Merge<D>::load(piece_of(k) + head * S::kStride + lane * Merge<D>::C, x[n]);
-        }
-#pragma unroll
-        for (int n = 0; n < 4; ++n) merge.add(x[n], scale[n]);
-      }
+      const Merge<D> merge = merged<D>(chain, weight, [&](int k) { return piece_of(k) + head * S::kStride + lane * Merge<D>::C; });
       const float sum = warp_sum(ml.y * weight);
       if (starts && ends) {
         merge.template write_out<T>(p, id, group, head, lane, sum);
@@ -857,6 +889,25 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) int4_attention_kern
         float* piece = scratch.cta_pieces + static_cast<int64_t>(2 * cta + (starts ? 1 : 0)) * S::kPiece;
         Merge<D>::store(piece + head * S::kStride + lane * Merge<D>::C, merge.o);
         if (lane == 0) *reinterpret_cast<float2*>(piece + S::kHeads * S::kStride + 2 * head) = make_float2(top, sum);
+      }
+    }
+  }
+
+  // the row of a cluster: its CTAs' pieces, a warp a head as before
+  if (parts > 1) {
+    cluster_sync();
+    const int from = lane < parts ? part_first(units, lane, parts) : 0, to = lane < parts ? part_first(units, lane + 1, parts) : 0;
+    const unsigned chain = __ballot_sync(0xffffffffu, from < to);
+    if (chain & (chain - 1)) {  // one CTA alone has written its row
+      const int first_cta = cta - rank, id = cta / parts;
+      auto cta_piece = [&](int k) { return scratch.cta_pieces + static_cast<int64_t>(2 * (first_cta + k) + (part_first(units, k, parts) == 0 ? 1 : 0)) * S::kPiece; };
+      for (int head = warp * parts + rank; head < group; head += kWarps * parts) {
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (from < to) ml = *reinterpret_cast<const float2*>(cta_piece(lane) + S::kHeads * S::kStride + 2 * head);
+        const float top = warp_max(ml.x);
+        const float weight = from < to ? fast_exp2(ml.x - top) : 0.f;
+        const Merge<D> merge = merged<D>(chain, weight, [&](int k) { return cta_piece(k) + head * S::kStride + lane * Merge<D>::C; });
+        merge.template write_out<T>(p, id, group, head, lane, warp_sum(ml.y * weight));
       }
     }
   }
@@ -940,6 +991,26 @@ int64_t scratch_bytes(int ctas) {
   return (pieces + 8 * ctas + 15) / 16 * 16;
 }
 
+// CTAs, a cluster, that hold a row each alone; 0: all CTAs share the places of all rows and the second
+// kernel joins rows that span some.  In units of a warp times two (0.85 us), of what rows as long as the
+// table take: a row's CTA starts and ends in about 3.2 us and those of a cluster in 5.5, with 1.7 for
+// every unit of a warp; the shares with the second kernel take 8.1 us and more.  Two sequences' rows (2 x
+// 128, 12 warps) of 128 tokens: 4.5 us on one CTA, 6.8 by shares; 513: 6.9, 8.1; 1024: 8.6, on four 7.2,
+// 8.2; 2048: on eight 7.5, 8.6; 4096: on eight 9.4, 9.0.  Lengths are not known here, so a row has its
+// own CTAs only where the longest possible rows take less than the shortest shares, unless the rows are
+// known to be about equally long.  More clusters of eight than 112 CTAs do not run at once, of four 128.
+int row_parts(int64_t rows, int64_t row_units, int warps, int ctas, bool even) {
+  auto warp_units = [&](int64_t units) { return (units + warps - 1) / warps; };
+  int64_t best = even ? 5 + 2 * warp_units((rows * (row_units + 1) + ctas - 1) / ctas) : 7;
+  int parts = 0;
+  for (int n = 1; n <= 8; n *= 2) {
+    if (rows * n > (n == 8 ? ctas * 3 / 4 : n > 1 ? ctas * 7 / 8 : ctas)) break;
+    const int64_t time = 2 * warp_units((row_units + n - 1) / n) + (n > 1 ? 3 : 0);
+    if (time < best) best = time, parts = n;
+  }
+  return parts;
+}
+
 template <typename T, int D, int NT>
 int launch(const PagedInt4& p, cudaStream_t stream) {
   using S = Shape<D, NT>;
@@ -955,12 +1026,22 @@ int launch(const PagedInt4& p, cudaStream_t stream) {
     QF_CUDA(cudaFuncSetAttribute(int4_attention_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     ready = device;
   }
+  const int64_t row_units = (p.table_width * p.page_size + kUnit - 1) / kUnit;
+  if (const int parts = row_parts(rows, row_units, S::kWarps, ctas, p.even); parts > 0) {
+    const dim3 grid(static_cast<unsigned>(rows * parts)), block(S::kThreads);
+    if (parts == 1) {
+      QF_CUDA(launch_chained(int4_attention_kernel<T, D, NT>, grid, block, static_cast<size_t>(S::kSmem), stream, p, 0, parts));
+    } else {
+      QF_CUDA(launch_chained(int4_attention_kernel<T, D, NT>, grid, block, static_cast<size_t>(S::kSmem), stream,
+                             ClusterShape{static_cast<unsigned>(parts), 1, 1}, p, 0, parts));
+    }
+    return QF_OK;
+  }
   const int chunk = static_cast<int>((rows + S::kThreads - 1) / S::kThreads);
-  QF_CUDA(launch_chained(int4_attention_kernel<T, D, NT>, dim3(ctas), dim3(S::kThreads), static_cast<size_t>(S::kSmem), stream, p, chunk));
+  QF_CUDA(launch_chained(int4_attention_kernel<T, D, NT>, dim3(ctas), dim3(S::kThreads), static_cast<size_t>(S::kSmem), stream, p, chunk, 0));
   // warps a head in the second kernel, four pieces each or more: a row is on all CTAs' share of the
   // rows at most, and on as many CTAs as its table has room for
   const int group = p.q_heads / p.kv_heads;
-  const int64_t row_units = (p.table_width * p.page_size + kUnit - 1) / kUnit;
   const int64_t row_ctas = std::min<int64_t>(ctas / rows, row_units / S::kWarps) / 4;
   const int each = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(row_ctas, group <= 8 ? 4 : 2)));
   QF_CUDA(launch_chained(int4_combine_kernel<T, D, NT>, dim3(ctas), dim3(32 * group * each), static_cast<size_t>(0), stream, p, ctas, each));

@@ -27,6 +27,7 @@ struct PagedInt4 {
   int table_dtype, lens_dtype;
   int new_tokens, take;
   Divisor by_heads, by_page, by_tiles;  // kv_heads, page_size, tiles of a page
+  bool even;   // rows are about equally long, most of them as long as the table
   bool early;  // table and lengths are step metadata: read before the kernel in front has finished
 };
 

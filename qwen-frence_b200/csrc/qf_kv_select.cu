@@ -66,6 +66,7 @@ int fill_paged_int4(const qf_paged_int4_args* a, int needs, PagedInt4* p) {
   r.batch = a->batch, r.q_heads = a->q_heads, r.kv_heads = a->kv_heads, r.page_size = a->page_size;
   r.table_dtype = a->table_dtype, r.lens_dtype = a->lens_dtype;
   r.new_tokens = a->new_tokens, r.take = a->take;
+  r.even = false;
   r.early = true;
   r.by_heads = make_divisor(a->kv_heads), r.by_page = make_divisor(a->page_size);
   r.by_tiles = make_divisor(a->page_size / kInt4Tile);
@@ -445,6 +446,7 @@ PagedInt4 over_selection(PagedInt4 p) {
   p.lens = p.page_lens, p.lens_dtype = QF_INDEX_I32;
   p.l_sb = p.kv_heads, p.l_sh = 1;
   p.early = false;  // the kernel in front writes both
+  p.even = true;
   return p;
 }
 

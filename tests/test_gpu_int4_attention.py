@@ -43,6 +43,35 @@ def test_splits(package, cuda_device, lengths):
     _check(package, cuda_device, q, pool, table, lens)
 
 
+@pytest.mark.parametrize("heads, group, dim, page", [(2, 6, 128, 16), (1, 16, 64, 32), (4, 4, 64, 16), (2, 9, 128, 16)])
+@pytest.mark.parametrize("batch, longest", [(1, 1), (1, 33), (2, 384), (1, 513), (3, 1024), (13, 1024), (14, 1024), (20, 1100), (1, 2000), (6, 2500), (7, 2500),
+                                            (37, 400), (38, 400), (74, 300), (75, 300), (148, 100), (149, 100)])
+def test_short_tables(package, cuda_device, batch, longest, heads, group, dim, page):
+    """Rows that one CTA or the CTAs of one cluster hold alone, and the sizes around them: no token, fewer
+    units than warps or CTAs, full rows; twice the same bits, then other lengths in the same tables."""
+    lengths = [longest, *([0, 1, longest // 2, 40, 33, 32, 31, longest - 1, longest] * batch)][:batch]
+    lengths = [min(n, longest) for n in lengths]
+    q, pool, table, lens = plain.make_cache(lengths, dim=dim, heads=heads, group=group, page=page, seed=batch)
+    out = _check(package, cuda_device, q, pool, table, lens)
+    assert torch.equal(out, _check(package, cuda_device, q, pool, table, lens))
+    _check(package, cuda_device, q, pool, table, lens // 3)
+
+
+@pytest.mark.parametrize("take, page", [(32, 64), (16, 32), (5, 16)])
+def test_choices_of_equal_length(package, cuda_device, take, page):
+    """The tables of a choice: most rows full, some short or empty."""
+    lengths = [page * take * 2 - 5] * 32
+    lengths[3], lengths[9], lengths[31] = 0, 1, page * take // 2
+    q, pool, table, lens = plain.make_cache(lengths, dtype=torch.bfloat16, page=page, seed=take)
+    k, v = plain.rows(pool, q.dtype)
+    limits = plain.bounds(k, table, lens, q.dtype, 10 ** 6, torch.zeros(pool.shape[0], 2, 2, 128, dtype=q.dtype))
+    for n in (32, 13, 1):
+        call = [t.to(cuda_device) for t in (q[:n], pool, limits, table[:n], lens[:n])]
+        out, pages, held = package.sparse_decode_attention_int4(*call, num_pages=take)
+        want, top = plain.attention(q[:n], k, v, pages.cpu(), held.cpu())
+        plain.assert_attention(out, want, top)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_magnitudes(package, cuda_device, dtype):
     """Values and queries far from one, scores far apart, one row far larger than the rest, and a scale of its own."""
