@@ -32,7 +32,7 @@
 // time, so issue and dependences bound it, and for short calls the way to the first tile (lengths, table,
 // tile: 3 us) and the launches.  64 sequences of 129..4097 tokens, 12 heads on 2 of 128: 18.4 us, 42 MB,
 // 2.3 TB/s; 256 of 64..4096, 16 on 4 of 64: 45.8 us, 172 MB, 3.8 TB/s; one of 513: 6.9 us (all in graphs).
-//  Warps an SM, measured before rows counted a place of their own, D = 128: 8 take 22 us for the
+// Warps an SM, measured before rows counted a place of their own, D = 128: 8 take 22 us for the
 // first, 10 22.3, 12 20.0, 14 20.9, 16 21.2 (from 13 on the registers no longer hold a row: 168 against 128 a
 // thread); D = 64: 12 take 54 us, 16 52, 20 54.
 // Taking the next unit's scores beside this one's values gives the schedulers two chains to choose from

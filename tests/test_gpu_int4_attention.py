@@ -240,6 +240,27 @@ def test_selection_of_ties_specials_and_many_pages(package, cuda_device):
     _selection(package, cuda_device, q[:1], limits, table, torch.tensor([many * 16 - 9]), many - 1, 16)
 
 
+@pytest.mark.parametrize("kind", ["wide", "near", "signs", "two values", "few bits", "huge", "one large"])
+@pytest.mark.parametrize("count", [2, 511, 1024, 2560, 2561, 9000])
+def test_selection_of_scores_of_all_kinds(package, cuda_device, kind, count):
+    """Scores that differ in their high bits, in their low ones, in sign, in one place, or not at all, at
+    the sizes where a thread holds more keys or none."""
+    g = torch.Generator().manual_seed(count)
+    x = torch.randn(count, 3, generator=g, dtype=torch.float64)
+    x = {"wide": lambda: x * torch.exp2(torch.randint(-12, 12, (count, 3), generator=g)), "signs": lambda: x.sign(),
+         "near": lambda: 1 + x.abs() * 0.01, "two values": lambda: (x > 0).double(), "huge": lambda: x * 6000,
+         "few bits": lambda: torch.cat([torch.full((count, 2), 512.0, dtype=torch.float64), x[:, :1].round() / 256], 1),
+         "one large": lambda: torch.where(torch.arange(count)[:, None] == count // 2, 100.0, 0.0) + torch.zeros(3)}[kind]()
+    limits = torch.zeros(count, 1, 2, 64)
+    limits[:, 0, :, 8] = x[:, :1]
+    limits[:, 0, :, 9], limits[:, 0, :, 40] = x[:, 1:2], x[:, 2:]
+    q = torch.zeros(1, 1, 64)
+    q[0, 0, [8, 9, 40]] = torch.tensor([1.0, 1.0, 2.0 ** -6])
+    table, lens = torch.randperm(count, generator=g)[None].int(), torch.tensor([count * 16 - 3], dtype=torch.int32)
+    for take in {1, 2, min(33, count), count // 2 + 1, count - 1} - {0}:
+        _selection(package, cuda_device, q.half(), limits.half(), table, lens, take, 16)
+
+
 def _decode_state(device, dtype=torch.float16, page=32, prompt=(200, 37, 90), steps=70):
     """Sequences with room to grow, their packed rows for a prompt and for every step."""
     g = torch.Generator().manual_seed(12)
