@@ -985,8 +985,14 @@ __global__ void __launch_bounds__(1024) int4_combine_kernel(const PagedInt4 p, i
   merge.template write_out<T>(p, row, group, head, lane, sum);
 }
 
+int64_t units_of_table(const PagedInt4& p) { return (p.table_width * p.page_size + kUnit - 1) / kUnit; }
+
+// None where row_parts() says one CTA a row for every smaller batch too: two units a warp at most.  (A
+// call that needs none is 2 us shorter on the host: nothing is allocated for it.)
 template <int D, int NT>
-int64_t scratch_bytes(int ctas) {
+int64_t scratch_bytes(const PagedInt4& p) {
+  const int ctas = sm_count();
+  if (static_cast<int64_t>(p.batch) * p.kv_heads <= ctas && units_of_table(p) <= 2 * Shape<D, NT>::kWarps) return 0;
   const int64_t pieces = static_cast<int64_t>(2 + Shape<D, NT>::kWarps) * ctas * Shape<D, NT>::kPiece * 4;
   return (pieces + 8 * ctas + 15) / 16 * 16;
 }
@@ -1016,8 +1022,8 @@ int launch(const PagedInt4& p, cudaStream_t stream) {
   using S = Shape<D, NT>;
   const int64_t rows = static_cast<int64_t>(p.batch) * p.kv_heads;
   const int ctas = sm_count();
-  const int64_t need = scratch_bytes<D, NT>(ctas);
-  QF_REQUIRE(p.workspace != nullptr && p.workspace_bytes >= need, "the workspace holds %lld bytes, %lld are needed",
+  const int64_t need = scratch_bytes<D, NT>(p);
+  QF_REQUIRE((p.workspace != nullptr || need == 0) && p.workspace_bytes >= need, "the workspace holds %lld bytes, %lld are needed",
              static_cast<long long>(p.workspace_bytes), static_cast<long long>(need));
   static thread_local int ready = -1;  // device whose kernel attribute this thread has set
   int device = 0;
@@ -1026,7 +1032,7 @@ int launch(const PagedInt4& p, cudaStream_t stream) {
     QF_CUDA(cudaFuncSetAttribute(int4_attention_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     ready = device;
   }
-  const int64_t row_units = (p.table_width * p.page_size + kUnit - 1) / kUnit;
+  const int64_t row_units = units_of_table(p);
   if (const int parts = row_parts(rows, row_units, S::kWarps, ctas, p.even); parts > 0) {
     const dim3 grid(static_cast<unsigned>(rows * parts)), block(S::kThreads);
     if (parts == 1) {
@@ -1076,9 +1082,8 @@ int sm_count() {
 
 int64_t int4_attention_bytes(const PagedInt4& p, int head_dim) {
   const bool two = p.q_heads / p.kv_heads > 8;
-  const int ctas = sm_count();
-  if (head_dim == 128) return two ? scratch_bytes<128, 2>(ctas) : scratch_bytes<128, 1>(ctas);
-  return two ? scratch_bytes<64, 2>(ctas) : scratch_bytes<64, 1>(ctas);
+  if (head_dim == 128) return two ? scratch_bytes<128, 2>(p) : scratch_bytes<128, 1>(p);
+  return two ? scratch_bytes<64, 2>(p) : scratch_bytes<64, 1>(p);
 }
 
 int launch_int4_attention(const PagedInt4& p, int head_dim, int dtype, cudaStream_t stream) {

@@ -539,7 +539,7 @@ int qf_int4_sparse_decode_attention(const qf_paged_int4_args* args, void* stream
   PagedInt4 next = over_selection(p);
   const int64_t keys = select_bytes(p);
   const int64_t more = int4_attention_bytes(next, args->head_dim);
-  QF_REQUIRE(p.workspace != nullptr && p.workspace_bytes >= keys + more, "the workspace holds %lld bytes, %lld are needed",
+  QF_REQUIRE((p.workspace != nullptr || keys + more == 0) && p.workspace_bytes >= keys + more, "the workspace holds %lld bytes, %lld are needed",
              static_cast<long long>(p.workspace_bytes), static_cast<long long>(keys + more));
   if (const int rc = launch_select(p, args->head_dim, args->dtype, s)) return rc;
   next.workspace = static_cast<uint8_t*>(p.workspace) + keys;

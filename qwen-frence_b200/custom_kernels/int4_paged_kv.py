@@ -341,8 +341,9 @@ def _run(function, call, device, batch, geometry, dtype, block_table, seq_lens, 
             if len(_workspace_sizes) >= 4096:
                 _workspace_sizes.clear()
             scratch_bytes = _workspace_sizes[key] = size.value
-        scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=block_table.device)
-        scratch_at = scratch.data_ptr()
+        if scratch_bytes:
+            scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=block_table.device)
+            scratch_at = scratch.data_ptr()
     _enqueue(function, (fill(),), device)
 
 

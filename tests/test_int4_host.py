@@ -115,6 +115,17 @@ def test_workspace_sizes(package):
     assert lib.qf_paged_int4_workspace(ctypes.byref(_paged_args(cabi)), cabi.INT4_SELECT, ctypes.byref(size)) == 0
     assert size.value == 2 * 2 * 8 * 4  # a 32-bit key for every page of every row
 
+    def attention(**changes):
+        assert lib.qf_paged_int4_workspace(ctypes.byref(_paged_args(cabi, **changes)), cabi.INT4_ATTENTION, ctypes.byref(size)) == 0
+        return size.value
+
+    # none for short tables, whatever the batch up to a row an SM; never more for a smaller call than for a larger one
+    assert attention(table_width=48) == attention(batch=74, table_width=48) == attention(table_width=0) == attention(batch=0) == 0
+    for sizes in (dict(head_dim=128), dict(head_dim=64), dict(head_dim=128, q_heads=20), dict(head_dim=64, q_heads=32)):
+        bytes_of = [[attention(batch=b, table_width=w, **sizes) for w in (1, 16, 32, 33, 48, 49, 64, 65, 200, 2048)] for b in (1, 8, 40, 74, 75, 300)]
+        for rows in (*bytes_of, *zip(*bytes_of)):
+            assert list(rows) == sorted(rows)
+
 
 def test_wrappers_refuse_before_any_device_work(package):
     pool = torch.zeros(4, 2, 1, 2560, dtype=torch.uint8)
