@@ -576,7 +576,8 @@ typedef struct qf_paged_int4_args {
 /* Scratch bytes of qf_int4_decode_attention, qf_select_kv_pages or
  * qf_int4_sparse_decode_attention (`call`, above) for these arguments on the current device.
  * Reads no device memory; nothing in the scratch needs clearing, and none of it may be shared
- * by calls that can overlap on the GPU. */
+ * by calls that can overlap on the GPU.  0 where a call needs none (workspace may then be null);
+ * what a call with larger batch or table_width needs is enough for a smaller one. */
 int qf_paged_int4_workspace(const qf_paged_int4_args* args, int32_t call, int64_t* bytes);
 
 /* out = softmax(scale * q k) v over every row's tokens; a row of length 0 gives zeros. */

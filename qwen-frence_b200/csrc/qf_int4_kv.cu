@@ -45,8 +45,8 @@ enum : int { kNoRope, kTable, kAngles };
 // row's 14 rotated heads hit the first level cache; passing them through shared memory instead costs
 // a barrier behind two dependent loads, 28 -> 22 us for 8192 rows); without a table the CTA computes
 // each once and shares it.  Bound by the latency of position -> table -> row and by issue: 8192 rows of
-// 12 + 2 + 2 x 128 take 17 us, 64 MB at 3.8 TB/s; with CTAs of 256 20 us, of 512 23 us, and with 12
-// CTAs an SM (40 registers) instead of 16 (32) 18 us.
+// 12 + 2 + 2 x 128 take 15.6 us, 64 MB at 4.1 TB/s; of 17 us, CTAs of 256 made 20, of 512 23, and 12
+// CTAs an SM (40 registers) instead of 16 (32) 18.
 template <typename T, int D, bool VEC, int ROPE>
 __global__ void __launch_bounds__(kWriteThreads, ROPE == kAngles ? 12 : 16) int4_write_kernel(const WriteParams p, const __grid_constant__ InvFreqTable freq) {
   constexpr int kHalf = D / 2, kLanes = D / 16, W = D / kInt4Group;
