@@ -597,7 +597,10 @@ int qf_int4_key_bounds(const qf_paged_int4_args* args, void* stream);
  * they hold -- a block table and lengths with head strides for qf_int4_decode_attention.  A
  * page id outside the pool scores below every other (one that 32 bits do not hold is -1 in
  * page_table).  Table and lengths are those of the
- * sequences.  batch * kv_heads at most 65535.  Ends with qf_order_next_launch(). */
+ * sequences.  batch * kv_heads at most 65535.  No kernel behind starts before both are
+ * written, and attention over a table with a head stride reads it behind its wait: choices
+ * and attentions of several streams, threads or devices may interleave.  Ends with
+ * qf_order_next_launch(). */
 int qf_select_kv_pages(const qf_paged_int4_args* args, void* stream);
 
 /* qf_select_kv_pages, then qf_int4_decode_attention over the pages it chose. */

@@ -1096,5 +1096,7 @@ extern "C" int qf_int4_decode_attention(const qf_paged_int4_args* args, void* st
   qf::PagedInt4 p;
   if (const int rc = qf::fill_paged_int4(args, qf::kNeedsQuery | qf::kNeedsPool | qf::kNeedsOut, &p)) return rc;
   if (p.batch == 0) return QF_OK;
+  // a table a KV head is what a choice of pages wrote: read behind the wait, whatever was launched since
+  p.early = p.t_sh == 0 && p.l_sh == 0;
   return qf::launch_int4_attention(p, args->head_dim, args->dtype, static_cast<cudaStream_t>(stream));
 }

@@ -28,7 +28,7 @@ struct PagedInt4 {
   int new_tokens, take;
   Divisor by_heads, by_page, by_tiles;  // kv_heads, page_size, tiles of a page
   bool even;   // rows are about equally long, most of them as long as the table
-  bool early;  // table and lengths are step metadata: read before the kernel in front has finished
+  bool early;  // table and lengths are step metadata: read before the kernel in front has finished; not those of a choice
 };
 
 enum : int { kNeedsQuery = 1, kNeedsPool = 2, kNeedsOut = 4, kNeedsBounds = 8, kNeedsSelection = 16 };

@@ -302,14 +302,16 @@ constexpr int kPickThreads = 512;
 // those that tie with the smallest as long as there is room.  A thread holds a run of kHeld neighbouring
 // keys and their pages in registers; longer rows are read again from the second level cache every time.
 // Bound by latency, loads and barriers: 2048 pages of one sequence take 6.7 us by themselves with the
-// launch; two bits at a time, counted in registers, took 10.6.
+// launch; two bits at a time, counted in registers, took 10.6.  `last`: the choice ends a call.  Kernels
+// behind may read table and lengths before they wait, so they start only when those are written; the
+// attention of a sparse call waits first and may stand by from the start.
 template <int kHeld>
-__global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const PagedInt4 p, const uint32_t* keys) {
+__global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const PagedInt4 p, const uint32_t* keys, bool last) {
   constexpr int kBins = 256, kPasses = 4;
   __shared__ __align__(16) int s_bins[kPasses][kBins];
   __shared__ uint32_t s_low[kPickThreads / 32], s_high[kPickThreads / 32];
   __shared__ int2 s_scan[kPickThreads / 32];
-  release_dependents();
+  if (!last) release_dependents();
   const int row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   for (int i = tid; i < kPasses * kBins; i += kPickThreads) (&s_bins[0][0])[i] = 0;
@@ -450,7 +452,7 @@ PagedInt4 over_selection(PagedInt4 p) {
   return p;
 }
 
-int launch_select(const PagedInt4& p, int head_dim, int dtype, cudaStream_t stream) {
+int launch_select(const PagedInt4& p, int head_dim, int dtype, bool last, cudaStream_t stream) {
   QF_REQUIRE((p.workspace != nullptr || select_bytes(p) == 0) && p.workspace_bytes >= select_bytes(p), "the workspace holds %lld bytes, %lld are needed",
              static_cast<long long>(p.workspace_bytes), static_cast<long long>(select_bytes(p)));
   const int rows = p.batch * p.kv_heads;
@@ -472,13 +474,13 @@ int launch_select(const PagedInt4& p, int head_dim, int dtype, cudaStream_t stre
   QF_CUDA(err);
   const uint32_t* scored = keys;
   if (p.table_width <= 2 * kPickThreads) {
-    err = launch_chained(page_pick_kernel<2>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored);
+    err = launch_chained(page_pick_kernel<2>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored, last);
   } else if (p.table_width <= 5 * kPickThreads) {
-    err = launch_chained(page_pick_kernel<5>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored);
+    err = launch_chained(page_pick_kernel<5>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored, last);
   } else if (p.table_width <= 16 * kPickThreads) {
-    err = launch_chained(page_pick_kernel<16>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored);
+    err = launch_chained(page_pick_kernel<16>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored, last);
   } else {
-    err = launch_chained(page_pick_kernel<0>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored);
+    err = launch_chained(page_pick_kernel<0>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored, last);
   }
   QF_CUDA(err);
   QF_CUDA(cudaGetLastError());
@@ -525,7 +527,7 @@ int qf_select_kv_pages(const qf_paged_int4_args* args, void* stream) {
   qf::PagedInt4 p;
   if (const int rc = qf::fill_paged_int4(args, qf::kNeedsQuery | qf::kNeedsBounds | qf::kNeedsSelection, &p)) return rc;
   if (p.batch == 0) return QF_OK;
-  if (const int rc = qf::launch_select(p, args->head_dim, args->dtype, static_cast<cudaStream_t>(stream))) return rc;
+  if (const int rc = qf::launch_select(p, args->head_dim, args->dtype, true, static_cast<cudaStream_t>(stream))) return rc;
   qf::request_ordered_launch();  // the selection is step metadata written by a kernel
   return QF_OK;
 }
@@ -541,7 +543,7 @@ int qf_int4_sparse_decode_attention(const qf_paged_int4_args* args, void* stream
   const int64_t more = int4_attention_bytes(next, args->head_dim);
   QF_REQUIRE((p.workspace != nullptr || keys + more == 0) && p.workspace_bytes >= keys + more, "the workspace holds %lld bytes, %lld are needed",
              static_cast<long long>(p.workspace_bytes), static_cast<long long>(keys + more));
-  if (const int rc = launch_select(p, args->head_dim, args->dtype, s)) return rc;
+  if (const int rc = launch_select(p, args->head_dim, args->dtype, false, s)) return rc;
   next.workspace = static_cast<uint8_t*>(p.workspace) + keys;
   next.workspace_bytes = p.workspace_bytes - keys;
   return launch_int4_attention(next, args->head_dim, args->dtype, s);
