@@ -443,6 +443,23 @@ struct Row {
     }
   }
 
+  // A NaN step as a step of 0 and a NaN floor: the sums of the weights, one product for all groups, stay
+  // finite, and the group is NaN by its floors' sum alone.  Returns the magnitude of what is left.
+  static __device__ __forceinline__ float keep_nans_apart(uint32_t (&vc)[4][W / 2], uint32_t (&ve)[4][W / 2], float largest_floor) {
+    float magnitude = fmaxf(largest_floor, 0.f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int j = 0; j < W / 2; ++j) {
+        const float2 step = unpack2<T>(vc[k][j]), floor = unpack2<T>(ve[k][j]);
+        ve[k][j] = pack2<T>(step.x == step.x ? floor.x : step.x, step.y == step.y ? floor.y : step.y);
+        vc[k][j] = pack2<T>(step.x == step.x ? step.x : 0.f, step.y == step.y ? step.y : 0.f);
+        magnitude = fmaxf(magnitude, fmaxf(step.x, step.y));
+      }
+    }
+    return magnitude;
+  }
+
   // Two tiles, `left` tokens of the row from their first on.
   __device__ __forceinline__ void unit(const uint8_t* smem, int left, int lane) {
     using V2 = typename Pair<T>::type;
@@ -473,11 +490,13 @@ struct Row {
     for (int k = 0; k < 4; ++k) {
 #pragma unroll
       for (int j = 0; j < W / 2; ++j) {
-        steps = __hmax2(steps, Pair<T>::of(vc[k][j]));
+        // a NaN step is kept where it must be seen: it takes the rare branch below
+        steps = kCentred ? __hmax2_nan(steps, Pair<T>::of(vc[k][j])) : __hmax2(steps, Pair<T>::of(vc[k][j]));
         floors = __hmax2(floors, __habs2(Pair<T>::of(ve[k][j])));
       }
     }
-    const float magnitude = fmaxf(fmaxf(to_float(steps.x), to_float(steps.y)), 0.015625f * fmaxf(to_float(floors.x), to_float(floors.y)));
+    const float largest_floor = 0.015625f * fmaxf(to_float(floors.x), to_float(floors.y));
+    float magnitude = kCentred ? max_nan(to_float(steps.x), to_float(steps.y), largest_floor) : fmaxf(fmaxf(to_float(steps.x), to_float(steps.y)), largest_floor);
     float a[NT][8];
     arguments(x, a, left, g);
     float top = a[0][0];
@@ -486,7 +505,10 @@ struct Row {
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = fmaxf(top, a[i][j]);
     }
-    if (__any_sync(0xffffffffu, (top > static_cast<float>(14 - e)) | (magnitude > pow2i(e)))) {
+    if (__any_sync(0xffffffffu, (top > static_cast<float>(14 - e)) | (kCentred ? !(magnitude <= pow2i(e)) : magnitude > pow2i(e)))) {
+      if constexpr (kCentred) {
+        if (__any_sync(0xffffffffu, magnitude != magnitude)) magnitude = keep_nans_apart(vc, ve, largest_floor);
+      }
       raise(x, magnitude, left, g);
       arguments(x, a, left, g);
     }

@@ -1,0 +1,59 @@
+"""GPU tests of the 4-bit cache at the edges of its definition."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import int4_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+def _spoil(pool, table, dtype, places):
+    """Make groups of V infinite: (sequence, token, KV head, group); the row's K and other groups stay as they read."""
+    page = pool.shape[2] * plain.TILE
+    k, v = plain.rows(pool, dtype)
+    for b, token, head, group in places:
+        ident, row = int(table[b, token // page]), token % page
+        kept_k, kept_v = (x[ident, row][None].to(dtype) for x in (k, v))
+        kept_v[0, head, 32 * group + 7] = float("inf")
+        plain.store(pool, torch.tensor([ident * page + row]), kept_k, kept_v)
+        k, v = plain.rows(pool, dtype)
+    return k, v
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads, group, dim, page", [(2, 6, 128, 16), (2, 4, 64, 32), (1, 16, 128, 16), (1, 12, 64, 16)])
+@pytest.mark.parametrize("longest", [1, 40, 700, 3000, 20000])
+def test_a_nan_group_of_v_stays_in_its_channels(package, cuda_device, dtype, heads, group, dim, page, longest):
+    """A group of V with an infinity reads back as NaN: 32 channels of the sequence's result are NaN, all others
+    are what they are without it, whether the row is one warp's, one CTA's, a cluster's or spread over CTAs."""
+    lengths = [longest, 33, longest, 5]
+    q, pool, table, lens = plain.make_cache(lengths, dtype=dtype, dim=dim, heads=heads, group=group, page=page, seed=longest)
+    last = dim // 32 - 1
+    places = [(0, longest // 2, 0, 0), (2, longest - 1, heads - 1, last), (1, 4, heads - 1, 1)]
+    k, v = _spoil(pool, table, dtype, places)
+    want, top = plain.attention(q, k, torch.nan_to_num(v, nan=0.0), table, lens)
+    out = package.paged_decode_attention_int4(*(t.to(cuda_device) for t in (q, pool, table, lens))).cpu()
+    spoiled = torch.zeros(out.shape, dtype=torch.bool)
+    for b, _, head, w in places:
+        spoiled[b, head * group:(head + 1) * group, 32 * w:32 * w + 32] = True
+    assert torch.equal(torch.isnan(out), spoiled)
+    plain.assert_attention(torch.where(spoiled, 0.0, out).to(dtype), torch.where(spoiled, 0.0, want), top)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_units_of_nan_groups(package, cuda_device, dtype):
+    """Whole units of 32 tokens whose V is NaN in one group, or in all of them in one sequence."""
+    q, pool, table, lens = plain.make_cache([200, 200, 64], dtype=dtype, seed=5)
+    places = [(0, t, 0, 2) for t in range(64, 96)] + [(1, t, 1, w) for t in range(32) for w in range(4)]
+    k, v = _spoil(pool, table, dtype, places)
+    want, top = plain.attention(q, k, torch.nan_to_num(v, nan=0.0), table, lens)
+    out = package.paged_decode_attention_int4(*(t.to(cuda_device) for t in (q, pool, table, lens))).cpu()
+    spoiled = torch.zeros(out.shape, dtype=torch.bool)
+    spoiled[0, :6, 64:96] = spoiled[1, 6:] = True
+    assert torch.equal(torch.isnan(out), spoiled)
+    plain.assert_attention(torch.where(spoiled, 0.0, out).to(dtype), torch.where(spoiled, 0.0, want), top)
