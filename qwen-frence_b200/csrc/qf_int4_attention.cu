@@ -255,8 +255,8 @@ struct Row {
   float off[NT][2];           // largest score so far (of the last raise) + e - 10
   int e;
 
-  // Query rows as fp16 with the largest element in [2^9, 2^10): a power of two, so exact but for
-  // elements 2^-20 below the largest.
+  // Query rows as fp16 with the largest element in [2^9, 2^10), of bf16 rows below 2^-117 less: a power
+  // of two, so exact but for elements 2^-20 below the largest.
   static __device__ __forceinline__ void load(const PagedInt4& p, int row, int group, int lane, uint4 (&raw)[NT][W]) {
     const int2 at = row_place(p, row);
     const T* src = static_cast<const T*>(p.q) + at.x * p.q_sb + static_cast<int64_t>(at.y) * group * p.q_sh + 8 * (lane & 3);
@@ -286,7 +286,7 @@ struct Row {
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int exponent = top > 0.f ? max(-100, min(100, 136 - (__float_as_int(top) >> 23))) : 0;
+      const int exponent = top > 0.f ? min(126, 136 - (__float_as_int(top) >> 23)) : 0;  // -119 for NaN and infinity
       const float up = pow2i(exponent);
       float sums[W];
 #pragma unroll

@@ -57,3 +57,14 @@ def test_units_of_nan_groups(package, cuda_device, dtype):
     spoiled[0, :6, 64:96] = spoiled[1, 6:] = True
     assert torch.equal(torch.isnan(out), spoiled)
     plain.assert_attention(torch.where(spoiled, 0.0, out).to(dtype), torch.where(spoiled, 0.0, want), top)
+
+
+@pytest.mark.parametrize("query", [1e36, 3e37, 1e-30, 1e-36])
+def test_queries_at_the_ends_of_bf16(package, cuda_device, query):
+    """bf16 queries of any magnitude whose scores are ordinary."""
+    q, pool, table, lens = plain.make_cache([40, 200, 1], dtype=torch.bfloat16, seed=2)
+    q = (q.float() * query).bfloat16()
+    scale = 0.1 / query
+    want, top = plain.attention(q, *plain.rows(pool, q.dtype), table, lens, scale)
+    out = package.paged_decode_attention_int4(*(t.to(cuda_device) for t in (q, pool, table, lens)), scale=scale)
+    plain.assert_attention(out, want, top)
