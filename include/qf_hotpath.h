@@ -330,6 +330,11 @@ int qf_device_status(int32_t* status, int32_t reset);
  * that arrives by a copy (the usual case) is ordered as usual; metadata that a
  * KERNEL updates in place on the same stream must be followed by
  * qf_order_next_launch() (qf_advance_decode_metadata does that itself).
+ * The 4-bit kernels: attention, page scores and choice read seq_lens and the block table in
+ * their set-up as well (attention not where the table has a head stride).  The write, the
+ * read-back and the bounds read nothing early and let the next kernel start only behind their
+ * own wait, so the launch that follows metadata a kernel updated may be one of those without
+ * a request, unless that kernel triggers dependent launches itself.
  * enabled == 0 launches everything the ordinary way (process-wide, read at launch
  * and capture time). */
 int qf_set_dependent_launch(int32_t enabled);

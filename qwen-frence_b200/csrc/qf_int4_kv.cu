@@ -50,10 +50,12 @@ enum : int { kNoRope, kTable, kAngles };
 template <typename T, int D, bool VEC, int ROPE>
 __global__ void __launch_bounds__(kWriteThreads, ROPE == kAngles ? 12 : 16) int4_write_kernel(const WriteParams p, const __grid_constant__ InvFreqTable freq) {
   constexpr int kHalf = D / 2, kLanes = D / 16, W = D / kInt4Group;
-  // The kernel behind may stand by early where this one leaves the SMs at once (64 rows, then attention
-  // of 64 sequences: 24.2 us, else 25.1), but not beside the CTAs of a long grid (8192 rows 20.9 us, else 21.6).
-  if (gridDim.x <= 148 * 16) release_dependents();
   dependency_wait();
+  // Behind the wait: attention reads lengths and tables before its own, and what the kernel in front of
+  // this one wrote is complete only now.
+  // The kernel behind may stand by early where this one leaves the SMs at once (64 rows, then attention
+  // of 64 sequences: 24.5 us, else 25.1), but not beside the CTAs of a long grid (8192 rows 20.9 us, else 21.6).
+  if (gridDim.x <= 148 * 16) release_dependents();
   const uint32_t first = blockIdx.x * kWriteThreads;
   const int index = first + threadIdx.x;
   const int row = quotient(index, p.items);
@@ -227,8 +229,8 @@ __global__ void __launch_bounds__(128) int4_read_kernel(const uint8_t* __restric
                                                         const Divisor kv_heads, const Divisor page_size,
                                                         T* __restrict__ k_out, T* __restrict__ v_out) {
   constexpr int W = D / kInt4Group;
-  release_dependents();
   dependency_wait();
+  release_dependents();  // behind the wait, as in the write
   const uint32_t segment = blockIdx.x * 32 + threadIdx.x / 4;
   const int t = threadIdx.x % 4;
   const int row = quotient(segment, kv_heads);

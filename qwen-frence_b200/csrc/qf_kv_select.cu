@@ -100,8 +100,8 @@ template <typename T, int D>
 __global__ void __launch_bounds__(32 * kBoundWarps) key_bounds_kernel(const PagedInt4 p, const Divisor by_each, int warps_each) {
   constexpr int W = D / kInt4Group, kWords = D / 8, kStep = 32 / kWords, kTokens = kInt4Tile / kStep;
   __shared__ float s_low[kBoundWarps][8][kWords], s_high[kBoundWarps][8][kWords];
-  release_dependents();
   dependency_wait();
+  release_dependents();  // behind the wait: scores and attention read lengths and tables before theirs
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int part = warp % warps_each;  // of the page's warps
   const uint32_t unit = blockIdx.x * (kBoundWarps / warps_each) + warp / warps_each;

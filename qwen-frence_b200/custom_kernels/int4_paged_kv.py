@@ -25,6 +25,13 @@ Long contexts: a query attends its newest page and the pages whose keys can scor
 
 Every call enqueues on the current stream of its tensors' device, reads nothing back and may be
 captured into a CUDA graph; scratch is a torch allocation of the call.  There is no CPU path.
+
+Block tables and lengths are step metadata: attention, scores and choice may read them while the
+kernel in front on the stream still runs.  Copies and torch ops that rewrite them need nothing more
+when a write, read or bounds call follows; in front of any other call of this library, ops that
+rewrite them in place are followed by qf_order_next_launch(), as for the 16-bit cache.  What
+select_kv_pages returns may go straight to paged_decode_attention_int4, whatever else is launched
+between them, on this stream or another.
 """
 
 from __future__ import annotations

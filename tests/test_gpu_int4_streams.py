@@ -130,3 +130,55 @@ def test_choices_and_attentions_of_two_threads(package, cuda_device):
     torch.cuda.synchronize()
     for got, want in zip(results, alone):
         assert len(got) == steps and all(torch.equal(a, b) for (_, a), b in zip(got, want))
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("between", ["write", "read", "bounds", "nothing", "advance"])
+def test_lengths_moved_on_by_a_kernel_in_front(package, cuda_device, between, captured):
+    """seq_lens.add_(1), as a decode loop does it, then a call, then attention: no copy and no request in between."""
+    batch, steps, first = 40, 60, 257
+    _, pool, table, lens = (t.to(cuda_device) for t in plain.make_cache([first + steps + 1] * batch, seed=7))
+    g = torch.Generator().manual_seed(7)
+    packed = (torch.randn(steps, batch, 2048, generator=g) * 0.7).half().to(cuda_device)
+    rope = plain.rope_table(400, 128).to(cuda_device)
+    limits = package.empty_key_bounds_int4(pool, torch.float16).zero_()
+    queries = torch.randn(steps, batch, 12, 128, generator=g).half().to(cuda_device)
+    positions = torch.full((batch,), first, device=cuda_device)
+    slots = table[:, first // 16].long() * 16 + first % 16
+
+    def run(wait):
+        """A copy of the cache, its steps one after another; the attention's results."""
+        cache, length, position, slot = pool.clone(), torch.full_like(lens, first), positions - int(between == "advance"), slots.clone()
+        bounds, results = limits.clone(), []
+        pause = torch.cuda.synchronize if wait else (lambda: None)
+        for step in range(steps):
+            if between == "advance":
+                package.advance_decode_state(position, length, slot, table, num_pages=cache.shape[0])
+            else:
+                length.add_(1)
+            pause()
+            if between in ("write", "advance"):
+                package.packed_qkv_rope_cache_int4(packed[step], position, slot, cache, rope_table=rope)
+            elif between == "read":
+                package.read_kv_int4(cache, slot, dtype=torch.float16)
+            elif between == "bounds":
+                package.update_key_bounds_int4(cache, bounds, table, length)
+            pause()
+            results.append(package.paged_decode_attention_int4(queries[step], cache, table, length))
+            if between == "bounds":
+                results.append(package.sparse_decode_attention_int4(queries[step], cache, bounds, table, length, num_pages=4)[1])
+            pause()
+        return results
+
+    want = run(True)
+    for _ in range(3):
+        if captured:
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                got = run(False)
+            graph.replay()
+        else:
+            got = run(False)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
