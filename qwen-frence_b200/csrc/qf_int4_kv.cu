@@ -221,13 +221,13 @@ __device__ __forceinline__ void load_elements(const uint8_t* at, float (&x)[W]) 
 // Rows at a list of slots as 16-bit K and V.  Four threads a row and head, eight channels of every
 // group each: seven loads bring a thread's D / 2 values, and its stores are 16 bytes beside its
 // neighbours' (16 threads a row, each with its own slot and addresses, were bound by those: 40 us for
-// 131072 rows of 2 x 128).  Bound by the stores: the 177 MB take 34 us, 5.2 TB/s.  A slot outside the
-// pool gives a row of zeros.
+// 131072 rows of 2 x 128).  Bound by the stores: the 177 MB take 32.6 us, 5.4 TB/s.  A slot outside the
+// pool gives a row of zeros.  Pool and slots may be written by the kernel in front: no __restrict__.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) int4_read_kernel(const uint8_t* __restrict__ pool, const void* __restrict__ slots,
+__global__ void __launch_bounds__(128) int4_read_kernel(const uint8_t* pool, const void* slots,
                                                         int slot_dtype, int64_t slot_stride, int rows, int64_t num_slots,
                                                         const Divisor kv_heads, const Divisor page_size,
-                                                        T* __restrict__ k_out, T* __restrict__ v_out) {
+                                                        T* k_out, T* v_out) {
   constexpr int W = D / kInt4Group;
   dependency_wait();
   release_dependents();  // behind the wait, as in the write
