@@ -4,7 +4,7 @@
 // written here equals, byte for byte, one computed with the same fp32 operations elsewhere.
 #include <cmath>
 
-#include "qf_int4_codec.cuh"
+#include "qf_int4_paged.cuh"
 #include "qf_rope_math.cuh"
 
 namespace qf {
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(128) int4_read_kernel(const uint8_t* pool, con
   }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned16(const void* p) { return on_boundary(p, 16); }
 
 bool good_geometry(int head_dim, int page_size) {
   return (head_dim == 64 || head_dim == 128) && page_size >= kInt4Tile && page_size % kInt4Tile == 0;
@@ -305,6 +305,10 @@ int launch_write(const qf_int4_write_args* a, cudaStream_t stream) {
   }
   QF_REQUIRE(a->slot_mapping == nullptr || a->slot_dtype == QF_INDEX_I32 || a->slot_dtype == QF_INDEX_I64,
              "slot mapping must use an integer dtype");
+  QF_REQUIRE(on_boundary(a->q, 2) && on_boundary(a->k, 2) && on_boundary(a->v, 2) && on_boundary(a->q_out, 2) &&
+                 index_aligned(a->positions, a->positions_dtype) && index_aligned(a->slot_mapping, a->slot_dtype) &&
+                 on_boundary(a->valid_tokens, 4),
+             "inputs must be aligned to their elements");
 
   WriteParams p{};
   p.q = a->q, p.k = a->k, p.v = a->v, p.q_out = a->q_out;
@@ -380,6 +384,7 @@ int qf_int4_read_rows(const void* pool, int64_t num_pages, int32_t page_size, in
   if (rows == 0) return QF_OK;
   QF_REQUIRE(pool && k_out && v_out, "pool, k_out and v_out must not be null");
   QF_REQUIRE(aligned16(pool) && aligned16(k_out) && aligned16(v_out), "pool and outputs must be 16-byte aligned");
+  QF_REQUIRE(index_aligned(slots, slot_dtype), "slots must be aligned to their elements");
   QF_REQUIRE(rows < (1LL << 31) / kv_heads - 256, "too many rows in one call");
   const dim3 grid(static_cast<unsigned>((rows * kv_heads + 31) / 32));
   cudaStream_t s = static_cast<cudaStream_t>(stream);

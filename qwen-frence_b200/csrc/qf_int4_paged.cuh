@@ -34,6 +34,8 @@ struct PagedInt4 {
 enum : int { kNeedsQuery = 1, kNeedsPool = 2, kNeedsOut = 4, kNeedsBounds = 8, kNeedsSelection = 16 };
 
 int fill_paged_int4(const qf_paged_int4_args* args, int needs, PagedInt4* p);
+inline bool on_boundary(const void* at, int bytes) { return (reinterpret_cast<uintptr_t>(at) & (bytes - 1)) == 0; }
+inline bool index_aligned(const void* at, int dtype) { return on_boundary(at, dtype == QF_INDEX_I64 ? 8 : 4); }
 // Multiprocessors of the current device, 148 where there is none.
 int sm_count();
 int64_t int4_attention_bytes(const PagedInt4& p, int head_dim);  // scratch of launch_int4_attention

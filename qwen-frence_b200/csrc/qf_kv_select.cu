@@ -31,10 +31,13 @@ int fill_paged_int4(const qf_paged_int4_args* a, int needs, PagedInt4* p) {
   }
   QF_REQUIRE(a->table_dtype == QF_INDEX_I32 || a->table_dtype == QF_INDEX_I64, "page table must use an integer dtype");
   QF_REQUIRE(a->lens_dtype == QF_INDEX_I32 || a->lens_dtype == QF_INDEX_I64, "lengths must use an integer dtype");
-  auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+  auto aligned = [](const void* x) { return on_boundary(x, 16); };
   if (a->batch > 0) {
     QF_REQUIRE(a->seq_lens && (a->block_table || a->table_width == 0), "block table and lengths must not be null");
+    QF_REQUIRE(index_aligned(a->block_table, a->table_dtype) && index_aligned(a->seq_lens, a->lens_dtype),
+               "block table and lengths must be aligned to their elements");
     if (needs & kNeedsQuery) {
+      QF_REQUIRE(aligned(a->workspace), "the workspace must be 16-byte aligned");
       QF_REQUIRE(a->q && aligned(a->q) && a->q_stride_b % 8 == 0 && a->q_stride_h % 8 == 0,
                  "q must be 16-byte aligned with strides of a multiple of 8 elements");
     }
@@ -52,6 +55,8 @@ int fill_paged_int4(const qf_paged_int4_args* a, int needs, PagedInt4* p) {
       QF_REQUIRE(static_cast<int64_t>(a->batch) * a->kv_heads * a->take < (1LL << 30) / (a->page_size / kInt4Tile),
                  "the pages taken hold 2^30 tiles of 16 tokens or more");
       QF_REQUIRE(a->page_table && a->page_lens, "page_table and page_lens must not be null");
+      QF_REQUIRE(index_aligned(a->page_table, QF_INDEX_I32) && index_aligned(a->page_lens, QF_INDEX_I32),
+                 "page_table and page_lens must be aligned to their elements");
     }
   }
   PagedInt4 r{};
