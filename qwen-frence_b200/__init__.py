@@ -97,14 +97,13 @@ def _load(key, path):
 
 def kernel_module(name):
     """One of the drop-in modules under custom_kernels/, loaded by path."""
-    return _load(f"qf_hotpath_{name}", KERNEL_DIR / f"{name}.py")
+    return sys.modules.get(f"qf_hotpath_{name}") or _load(f"qf_hotpath_{name}", KERNEL_DIR / f"{name}.py")
 
 
 def __getattr__(name):
-    if name in _EXPORTS:
-        # kept, so that a call does not look its module up again
-        value = globals()[name] = getattr(kernel_module(_EXPORTS[name]), name)
-        return value
+    module = _EXPORTS.get(name)
+    if module is not None:  # looked up every time: a function replaced on its module is the package's too
+        return getattr(kernel_module(module), name)
     if name == "cabi":
         # one shared instance with the drop-in modules, which load it by path
         return _load("qf_hotpath_cabi", PACKAGE_DIR / "_cabi.py")

@@ -61,3 +61,15 @@ def test_inputs_of_reads_and_writes_are_aligned_to_their_elements(package):
             setattr(args, name, value)
         assert lib.qf_int4_rope_kv_write(ctypes.byref(args), None) == -1
         assert b"aligned to their elements" in lib.qf_last_error(), changes
+
+
+@pytest.mark.parametrize("name, module", [("rms_norm", "fused_rms"), ("packed_qkv_rope_cache", "packed_qkv_rope_cache"),
+                                          ("paged_decode_attention_int4", "int4_paged_kv")])
+def test_the_package_hands_out_what_its_modules_hold(package, monkeypatch, name, module):
+    """A function replaced on a drop-in module is the package's, before and after."""
+    before = getattr(package, name)
+    stand_in = object()
+    monkeypatch.setattr(package.kernel_module(module), name, stand_in)
+    assert getattr(package, name) is stand_in
+    monkeypatch.undo()
+    assert getattr(package, name) is before is getattr(package.kernel_module(module), name)
