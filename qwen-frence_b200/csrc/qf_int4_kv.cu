@@ -292,7 +292,7 @@ int launch_write(const qf_int4_write_args* a, cudaStream_t stream) {
   const int items = (a->q_heads + 2 * a->kv_heads) * (a->head_dim / 16);
   QF_REQUIRE(a->q_heads < (1 << 20) && a->kv_heads < (1 << 20) && static_cast<int64_t>(a->rows) * items < (1LL << 31) - kWriteThreads,
              "too many rows in one call");
-  QF_REQUIRE(a->k && a->v && a->pool, "k, v and the pool must not be null");
+  QF_REQUIRE(a->k && a->v && (a->pool || a->num_pages == 0), "k, v and the pool must not be null");
   QF_REQUIRE(a->q_heads == 0 || (a->q && a->q_out), "q and q_out are required with query heads");
   QF_REQUIRE(aligned16(a->pool), "the pool must be 16-byte aligned");
   if (a->positions != nullptr) {
@@ -382,7 +382,7 @@ int qf_int4_read_rows(const void* pool, int64_t num_pages, int32_t page_size, in
   QF_REQUIRE(slots == nullptr || slot_dtype == QF_INDEX_I32 || slot_dtype == QF_INDEX_I64,
              "slot mapping must use an integer dtype");
   if (rows == 0) return QF_OK;
-  QF_REQUIRE(pool && k_out && v_out, "pool, k_out and v_out must not be null");
+  QF_REQUIRE((pool || num_pages == 0) && k_out && v_out, "pool, k_out and v_out must not be null");
   QF_REQUIRE(aligned16(pool) && aligned16(k_out) && aligned16(v_out), "pool and outputs must be 16-byte aligned");
   QF_REQUIRE(index_aligned(slots, slot_dtype), "slots must be aligned to their elements");
   QF_REQUIRE(rows < (1LL << 31) / kv_heads - 256, "too many rows in one call");

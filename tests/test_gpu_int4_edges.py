@@ -68,3 +68,18 @@ def test_queries_at_the_ends_of_bf16(package, cuda_device, query):
     want, top = plain.attention(q, *plain.rows(pool, q.dtype), table, lens, scale)
     out = package.paged_decode_attention_int4(*(t.to(cuda_device) for t in (q, pool, table, lens)), scale=scale)
     plain.assert_attention(out, want, top)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pools_without_pages_are_read_and_written(package, cuda_device, dtype):
+    """Every slot is outside a pool without pages: zeros are read, nothing is written, queries are rotated."""
+    pool = package.empty_kv_pool_int4(0, 2, 128, device=cuda_device)
+    slots = torch.tensor([0, 5, -1], device=cuda_device)
+    for x in package.read_kv_int4(pool, slots, dtype=dtype):
+        assert x.shape == (3, 2, 128) and (x == 0).all()
+    for x in package.dequantize_kv_pool_int4(pool, dtype):
+        assert x.shape == (0, 16, 2, 128)
+    packed = torch.randn(3, 2048, device=cuda_device).to(dtype)
+    rope = plain.rope_table(10, 128)
+    q = package.packed_qkv_rope_cache_int4(packed, slots.clamp(min=0), slots, pool, rope_table=rope.to(cuda_device))
+    assert torch.equal(q.cpu(), plain.rope(packed.cpu().view(3, 16, 128)[:, :12], rope, slots.cpu().clamp(min=0)))
