@@ -421,9 +421,11 @@ def update_key_bounds_int4(kv4_pool, key_bounds, block_table, seq_lens, *, new_t
     return key_bounds
 
 
-def _check_take(num_pages):
-    _require(isinstance(num_pages, int) and not isinstance(num_pages, bool) and 1 <= num_pages < 2 ** 31,
-             "num_pages must be a positive integer")
+def _check_take(num_pages, rows, page_size):
+    """Before the choice is allocated: a row of it holds fewer than 2^30 tokens, all rows fewer than 2^30 tiles."""
+    _require(isinstance(num_pages, int) and not isinstance(num_pages, bool) and 1 <= num_pages, "num_pages must be a positive integer")
+    _require(num_pages < 2 ** 30 // page_size and rows * num_pages < 2 ** 30 // (page_size // TILE_TOKENS),
+             "num_pages is too large: a choice holds fewer than 2^30 tokens a row and 2^30 tiles of 16 in all")
 
 
 def _empty_choice(batch, kv_heads, num_pages, device):
@@ -444,7 +446,7 @@ def select_kv_pages(q, key_bounds, block_table, seq_lens, *, num_pages, page_siz
     pages, kv_heads, _, dim = key_bounds.shape
     geometry = (pages, kv_heads, dim, page_size)
     q = _check_query(q, geometry)
-    _check_take(num_pages)
+    _check_take(num_pages, q.shape[0] * kv_heads, page_size)
     device = key_bounds.get_device()
     _require(q.get_device() == device, _PAGED_DEVICE)
     choice = _empty_choice(q.shape[0], kv_heads, num_pages, q.device)
@@ -460,7 +462,7 @@ def sparse_decode_attention_int4(q, kv4_pool, key_bounds, block_table, seq_lens,
     dtype = _element_code(q.dtype)
     _check_bounds(key_bounds, q.dtype, geometry)
     q = _check_query(q, geometry)
-    _check_take(num_pages)
+    _check_take(num_pages, q.shape[0] * geometry[1], geometry[3])
     device = kv4_pool.get_device()
     _require(q.get_device() == device and key_bounds.get_device() == device, _PAGED_DEVICE)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)

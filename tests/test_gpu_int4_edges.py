@@ -83,3 +83,18 @@ def test_pools_without_pages_are_read_and_written(package, cuda_device, dtype):
     rope = plain.rope_table(10, 128)
     q = package.packed_qkv_rope_cache_int4(packed, slots.clamp(min=0), slots, pool, rope_table=rope.to(cuda_device))
     assert torch.equal(q.cpu(), plain.rope(packed.cpu().view(3, 16, 128)[:, :12], rope, slots.cpu().clamp(min=0)))
+
+
+@pytest.mark.parametrize("num_pages", [2 ** 31 - 1, 2 ** 26, 2 ** 62, 0, True])
+def test_choices_too_large_are_refused_before_they_are_allocated(package, cuda_device, num_pages):
+    """16 rows: 2^30 tiles over 16 rows and one tile a page leave fewer than 2^26 pages a row."""
+    q, pool, table, lens = (t.to(cuda_device) for t in plain.make_cache([64] * 8))
+    limits = package.empty_key_bounds_int4(pool, q.dtype).zero_()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    for call in (lambda: package.select_kv_pages(q, limits, table, lens, num_pages=num_pages),
+                 lambda: package.sparse_decode_attention_int4(q, pool, limits, table, lens, num_pages=num_pages)):
+        with pytest.raises(ValueError, match="num_pages"):
+            call()
+    assert torch.cuda.max_memory_allocated() - before < 2 ** 20
