@@ -10,9 +10,11 @@
 // floors are one more product.  With p = exp2(s - offset) and V codes m, steps c, floors e,
 //     o[d, h] = sum_t (p[t, h] c[t, w(d)]) m[t, d] + sum_t p[t, h] e[t, w(d)]
 // where p c is rounded to fp16 (2^-11 of a weight at most; products and sums are fp32).  The offset is
-// the running maximum of s, plus the exponent of the largest c, less 10, so that p c stays below 2^15
-// and keeps fp16's precision down to 2^-24 of the largest weight, whatever the magnitude of V; it is
-// raised, and the sums rescaled, only when a score or a step exceeds what the last offset allows by 2^4.
+// the running maximum of s, plus the exponent of the largest c (or of |e| / 64 where that is larger), less
+// 10, so that p c stays below 2^15; it is raised, and the sums rescaled, only when a score or a step exceeds
+// what the last offset allows by 2^4.  One exponent serves all groups of the tokens that a warp has seen of
+// a row: in a group whose steps are 2^-k of the largest, p c keeps fp16's precision down to 2^-(24 - k) of
+// the largest weight; below that it is off by at most 2^-25, where the largest p c is 2^10.
 //
 // Work.  Rows are laid end to end as units of two tiles and every CTA, one an SM, takes an equal share
 // of them, every warp of the CTA an equal share of that, whatever rows it covers.  A warp streams its
@@ -27,11 +29,11 @@
 //
 // Bound.  The cache's 5 bits a channel come in at the memory's rate only if the SM spends no more than
 // 110 cycles on a tile of D = 128 (55 at D = 64); it issues about 250 (200) instructions a tile, a third
-// of them the masks and shifts that take codes apart, on four schedulers of which each is busy six
-// cycles in ten.  With all tiles in one page, that is with no memory to wait for, calls take 7 % less
+// of them the masks and shifts that take codes apart, on four schedulers of which each issues in 46 (D
+// 64: 62) cycles of a hundred.  With all tiles in one page, that is with no memory to wait for, calls take 7 % less
 // time, so issue and dependences bound it, and for short calls the way to the first tile (lengths, table,
 // tile: 3 us) and the launches.  64 sequences of 129..4097 tokens, 12 heads on 2 of 128: 18.4 us, 42 MB,
-// 2.3 TB/s; 256 of 64..4096, 16 on 4 of 64: 45.8 us, 172 MB, 3.8 TB/s; one of 513: 6.9 us (all in graphs).
+// 2.3 TB/s; 256 of 64..4096, 16 on 4 of 64: 45.8 us, 172 MB, 3.8 TB/s; one of 513: 7.0 us (all in graphs).
 // Warps an SM, measured before rows counted a place of their own, D = 128: 8 take 22 us for the
 // first, 10 22.3, 12 20.0, 14 20.9, 16 21.2 (from 13 on the registers no longer hold a row: 168 against 128 a
 // thread); D = 64: 12 take 54 us, 16 52, 20 54.

@@ -1,7 +1,7 @@
 // The 4-bit paged KV cache: layout of a tile and the codec of a group.
 //
 // A tile holds 16 tokens of one KV head, K and V together, in 20 * D bytes (D = 64 or 128):
-// one contiguous block, so one bulk copy brings everything a warp needs for 16 tokens.
+// one contiguous block, which a warp fetches whole, 16 bytes a lane side by side.
 // Every 32 consecutive channels of a row are a group with a step and a floor in the element
 // type T of the queries; a channel is a code n in 0..15 and stands for n * step + floor:
 //     floor = min(x),  step = T((max(x) - min(x)) / 15),  n = rint((x - floor) / step)

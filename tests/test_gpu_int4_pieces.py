@@ -82,3 +82,28 @@ def test_every_chosen_page_is_counted_once(package, cuda_device, dtype, take):
             parts = pieces.weighted(q[b, mine].to(cuda_device), k[ids, :, h].flatten(0, 1), v[ids, :, h].flatten(0, 1), n, 128 ** -0.5)
             for got in (out, again):
                 assert ((got[b, mine].double() - parts[0]).abs() / pieces.bound(dtype, *parts)).max() <= 1.0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads, group, dim, page", LAYOUTS)
+@pytest.mark.parametrize("factor", [2.0 ** -6, 2.0 ** -10, 2.0 ** -14])
+def test_groups_of_unlike_steps(package, cuda_device, dtype, heads, group, dim, page, factor):
+    """Groups of V whose steps are far below another group's, an early token far above the rest, values of one
+    sign and a large offset, and scores with a peak and a long tail: every channel within its own group's bound and
+    2^-30 a token of the largest step's range."""
+    lengths = [3000, 700, 40]
+    q, pool, table, lens = plain.make_cache(lengths, dtype=dtype, dim=dim, heads=heads, group=group, page=page, seed=3)
+    g = torch.Generator().manual_seed(3)
+    for b, n in enumerate(lengths):
+        token = torch.arange(n)
+        slots = table[b, token // page].long() * page + token % page
+        v = torch.randn(n, heads, dim, generator=g)
+        v[..., : dim // 2] *= 8.0
+        v[..., dim // 2:] *= 8.0 * factor
+        v[n // 2, :, :32] *= 4.0
+        v[..., dim - 32:] = v[..., dim - 32:].abs() + 50.0 * factor
+        k = torch.randn(n, heads, dim, generator=g) * 0.3
+        plain.store_fast(pool, slots, k.to(dtype), v.to(dtype))
+    for scale in (0.02, 0.3, 2.0):
+        out = _attend(package, cuda_device, q, pool, table, lens, scale=scale)
+        assert pieces.worst(out, *pieces.expected(q, pool, table, lens, scale, device=cuda_device)) <= 1.0
