@@ -31,12 +31,14 @@ struct WriteParams {
   Divisor items, page_size;
   int rows, q_heads, kv_heads, table_positions;
   int pos_dtype, slot_dtype;
+  bool one_wave;  // the grid is resident at once
 };
 
 constexpr int kWriteThreads = 128;
 
 // Where the angles of a call come from.
 enum : int { kNoRope, kTable, kAngles };
+constexpr int write_ctas(int rope) { return rope == kAngles ? 12 : 16; }  // an SM
 
 // Rows and their segments (heads) are laid end to end: a segment takes D / 16 threads, each with
 // the eight channels at d0 and the eight they rotate with at d0 + D / 2, so a CTA of 128 covers a row
@@ -48,14 +50,14 @@ enum : int { kNoRope, kTable, kAngles };
 // 12 + 2 + 2 x 128 take 15.6 us, 64 MB at 4.1 TB/s; of 17 us, CTAs of 256 made 20, of 512 23, and 12
 // CTAs an SM (40 registers) instead of 16 (32) 18.
 template <typename T, int D, bool VEC, int ROPE>
-__global__ void __launch_bounds__(kWriteThreads, ROPE == kAngles ? 12 : 16) int4_write_kernel(const WriteParams p, const __grid_constant__ InvFreqTable freq) {
+__global__ void __launch_bounds__(kWriteThreads, write_ctas(ROPE)) int4_write_kernel(const WriteParams p, const __grid_constant__ InvFreqTable freq) {
   constexpr int kHalf = D / 2, kLanes = D / 16, W = D / kInt4Group;
   dependency_wait();
   // Behind the wait: attention reads lengths and tables before its own, and what the kernel in front of
   // this one wrote is complete only now.
   // The kernel behind may stand by early where this one leaves the SMs at once (64 rows, then attention
   // of 64 sequences: 24.5 us, else 25.1), but not beside the CTAs of a long grid (8192 rows 20.9 us, else 21.6).
-  if (gridDim.x <= 148 * 16) release_dependents();
+  if (p.one_wave) release_dependents();
   const uint32_t first = blockIdx.x * kWriteThreads;
   const int index = first + threadIdx.x;
   const int row = quotient(index, p.items);
@@ -336,6 +338,7 @@ int launch_write(const qf_int4_write_args* a, cudaStream_t stream) {
           mult8(a->q_stride_row) && mult8(a->q_stride_head) && mult8(a->o_stride_row) && mult8(a->o_stride_head);
   }
   const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a->rows) * items + kWriteThreads - 1) / kWriteThreads));
+  p.one_wave = grid.x <= static_cast<unsigned>(sm_count() * write_ctas(a->positions == nullptr ? kNoRope : a->rope_table != nullptr ? kTable : kAngles));
   cudaError_t err = cudaSuccess;
 #define QF_LAUNCH_WRITE_AS(T, D, ROPE)                                                                              \
   err = vec ? launch_chained(int4_write_kernel<T, D, true, ROPE>, grid, dim3(kWriteThreads), 0, stream, p, freq)     \
