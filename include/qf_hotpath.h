@@ -591,7 +591,7 @@ int qf_int4_decode_attention(const qf_paged_int4_args* args, void* stream);
 /* key_bounds of every page that holds one of the last `new_tokens` tokens of its sequence,
  * over the page's tokens below the sequence's length; other pages keep theirs.  Table and
  * lengths are those of the sequences (the head strides are not used).  A NaN key makes both
- * bounds of its channel NaN. */
+ * bounds of its channel NaN.  Sequences that share a page hold the same number of its tokens. */
 int qf_int4_key_bounds(const qf_paged_int4_args* args, void* stream);
 
 /* The pages every row attends: its newest page and the take - 1 others with the highest
@@ -608,7 +608,7 @@ int qf_int4_key_bounds(const qf_paged_int4_args* args, void* stream);
  * qf_order_next_launch(). */
 int qf_select_kv_pages(const qf_paged_int4_args* args, void* stream);
 
-/* qf_select_kv_pages, then qf_int4_decode_attention over the pages it chose. */
+/* qf_select_kv_pages, then qf_int4_decode_attention over the pages it chose; scale not negative. */
 int qf_int4_sparse_decode_attention(const qf_paged_int4_args* args, void* stream);
 
 /* Switches for tests and experiments (process-wide, read at launch time).

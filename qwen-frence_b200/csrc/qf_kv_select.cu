@@ -540,6 +540,7 @@ int qf_select_kv_pages(const qf_paged_int4_args* args, void* stream) {
 int qf_int4_sparse_decode_attention(const qf_paged_int4_args* args, void* stream) {
   using namespace qf;
   PagedInt4 p;
+  QF_REQUIRE(args == nullptr || !(args->scale < 0.f), "scale must not be negative: pages are chosen by their largest scores");
   if (const int rc = fill_paged_int4(args, kNeedsQuery | kNeedsPool | kNeedsOut | kNeedsBounds | kNeedsSelection, &p)) return rc;
   if (p.batch == 0) return QF_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -276,8 +276,9 @@ def _read(kv4_pool, slots, rows, dtype):
 
 
 def read_kv_int4(kv4_pool, slot_mapping, *, dtype=None):
-    """Rows of the cache at a list of slots as (k, v), both [n, Hkv, D] in `dtype` (that of the
-    writes; default float16).  A slot outside the pool, -1 for one, gives a row of zeros."""
+    """Rows of the cache at a list of slots as (k, v), both [n, Hkv, D] in `dtype`, that of the writes,
+    which the pool does not hold: steps and floors read as another type are other numbers (default
+    float16).  A slot outside the pool, -1 for one, gives a row of zeros."""
     shape = slot_mapping.shape
     if len(shape) != 1:
         raise ValueError("slot mapping must be a list of slots")
@@ -288,7 +289,8 @@ def read_kv_int4(kv4_pool, slot_mapping, *, dtype=None):
 
 
 def dequantize_kv_pool_int4(kv4_pool, dtype=None):
-    """The whole cache as 16-bit pools (k_pool, v_pool), both [pages, page_size, Hkv, D]."""
+    """The whole cache as 16-bit pools (k_pool, v_pool), both [pages, page_size, Hkv, D], in `dtype`: that
+    of the writes, as for read_kv_int4."""
     pages, kv_heads, dim, page_size = _check_pool(kv4_pool)
     k, v = _read(kv4_pool, (None, 0, 0), pages * page_size, torch.float16 if dtype is None else dtype)
     shape = (pages, page_size, kv_heads, dim)
@@ -408,7 +410,8 @@ def update_key_bounds_int4(kv4_pool, key_bounds, block_table, seq_lens, *, new_t
     (1 after a decode step, the prompt's length after a prefill); returns key_bounds.
 
     Bounds are the smallest and the largest key of a page's tokens below seq_lens, per channel, as the
-    cache reads back."""
+    cache reads back.  Sequences that share a page hold the same number of its tokens: one that holds
+    more might find the bounds of fewer."""
     geometry = _check_pool(kv4_pool)
     dtype = _element_code(key_bounds.dtype)
     _check_bounds(key_bounds, key_bounds.dtype, geometry)
@@ -439,7 +442,9 @@ def select_kv_pages(q, key_bounds, block_table, seq_lens, *, num_pages, page_siz
 
     A row is the sequence's newest page and the num_pages - 1 others with the highest bound on a score,
     the largest over the KV head's query heads of sum_d max(q_d * low_d, q_d * high_d); ties go to the
-    earlier page.  Pages keep the sequence's order; -1 pads a sequence that has fewer."""
+    earlier page.  Pages keep the sequence's order; -1 pads a sequence that has fewer.  page_size is the
+    pool's, kv4_pool.shape[2] * 16: the bounds do not hold it, and with another one every length is cut
+    into other pages."""
     dtype = _element_code(q.dtype)
     _check_bounds(key_bounds, q.dtype)
     _require(page_size >= TILE_TOKENS and page_size % TILE_TOKENS == 0, "page_size must be a multiple of 16")
@@ -457,8 +462,10 @@ def select_kv_pages(q, key_bounds, block_table, seq_lens, *, num_pages, page_siz
 
 def sparse_decode_attention_int4(q, kv4_pool, key_bounds, block_table, seq_lens, *, num_pages, scale=None):
     """select_kv_pages and paged_decode_attention_int4 over its choice in one call: (out, page_table,
-    page_lens).  key_bounds must be up to date for every page but a sequence's newest."""
+    page_lens).  key_bounds must be up to date for every page but a sequence's newest.  The pages are
+    those of the largest q . k, so scale is not negative."""
     geometry = _check_pool(kv4_pool)
+    _require(scale is None or scale >= 0, "scale must not be negative: pages are chosen by their largest scores")
     dtype = _element_code(q.dtype)
     _check_bounds(key_bounds, q.dtype, geometry)
     q = _check_query(q, geometry)

@@ -98,3 +98,15 @@ def test_choices_too_large_are_refused_before_they_are_allocated(package, cuda_d
         with pytest.raises(ValueError, match="num_pages"):
             call()
     assert torch.cuda.max_memory_allocated() - before < 2 ** 20
+
+
+def test_sparse_attention_takes_scales_from_zero_on(package, cuda_device):
+    q, pool, table, lens = plain.make_cache([300, 64])
+    k, v = plain.rows(pool, q.dtype)
+    limits = plain.bounds(k, table, lens, q.dtype, 10 ** 6, torch.zeros(pool.shape[0], 2, 2, 128, dtype=q.dtype))
+    call = [t.to(cuda_device) for t in (q, pool, limits, table, lens)]
+    for scale in (0.0, 0.3):
+        out, pages, held = package.sparse_decode_attention_int4(*call, num_pages=5, scale=scale)
+        plain.assert_attention(out, *plain.attention(q, k, v, pages.cpu(), held.cpu(), scale))
+    with pytest.raises(ValueError, match="scale"):
+        package.sparse_decode_attention_int4(*call, num_pages=5, scale=-0.3)

@@ -73,3 +73,11 @@ def test_the_package_hands_out_what_its_modules_hold(package, monkeypatch, name,
     assert getattr(package, name) is stand_in
     monkeypatch.undo()
     assert getattr(package, name) is before is getattr(package.kernel_module(module), name)
+
+
+def test_sparse_attention_refuses_a_negative_scale(package):
+    """Its pages are those of the largest q . k, which a negative scale would make the smallest scores."""
+    lib = package.cabi.library()
+    assert lib.qf_int4_sparse_decode_attention(ctypes.byref(_sparse_args(package.cabi, scale=-0.1)), None) == -1
+    assert b"scale" in lib.qf_last_error()
+    assert lib.qf_int4_sparse_decode_attention(ctypes.byref(_sparse_args(package.cabi, batch=0, scale=0.0)), None) == 0
