@@ -29,11 +29,11 @@
 //
 // Bound.  The cache's 5 bits a channel come in at the memory's rate only if the SM spends no more than
 // 110 cycles on a tile of D = 128 (55 at D = 64); it issues about 250 (200) instructions a tile, a third
-// of them the masks and shifts that take codes apart, on four schedulers of which each issues in 46 (D
-// 64: 62) cycles of a hundred.  With all tiles in one page, that is with no memory to wait for, calls take 7 % less
+// of them the masks and shifts that take codes apart, on four schedulers of which each issues in 47 (D
+// 64: 63) cycles of a hundred.  With all tiles in one page, that is with no memory to wait for, calls take 7 % less
 // time, so issue and dependences bound it, and for short calls the way to the first tile (lengths, table,
-// tile: 3 us) and the launches.  64 sequences of 129..4097 tokens, 12 heads on 2 of 128: 18.4 us, 42 MB,
-// 2.3 TB/s; 256 of 64..4096, 16 on 4 of 64: 45.8 us, 172 MB, 3.8 TB/s; one of 513: 7.0 us (all in graphs).
+// tile: 3 us) and the launches.  64 sequences of 129..4097 tokens, 12 heads on 2 of 128: 18.5 us, 42 MB,
+// 2.3 TB/s; 256 of 64..4096, 16 on 4 of 64: 45.6 us, 172 MB, 3.8 TB/s; one of 513: 7.0 us (all in graphs).
 // Warps an SM, measured before rows counted a place of their own, D = 128: 8 take 22 us for the
 // first, 10 22.3, 12 20.0, 14 20.9, 16 21.2 (from 13 on the registers no longer hold a row: 168 against 128 a
 // thread); D = 64: 12 take 54 us, 16 52, 20 54.
@@ -245,7 +245,10 @@ struct Row {
   static constexpr int W = D / kInt4Group;
   // A rounded weight is off by 2^-12 of itself on average, times a code of 7.5 on average.  For fp16
   // results the codes count from 7.5: sum_t (p c) m = sum_t fl(p c) (m - 7.5) + 7.5 sum_t p c but for the
-  // rounding of fl, now times |m - 7.5|.  bf16 results are rounded coarser than either.
+  // rounding of fl, now times |m - 7.5|.  bf16 results are rounded coarser than either: they differ from an
+  // fp32 attention's by 1.3e-4 to 2.4e-4 of their norm, a last place here and there, and are as far from the exact
+  // ones as those (1.5e-3); centred codes would make that 0.9e-4 to 1.9e-4 and 256 sequences of 64..4096 tokens
+  // (D 64) 49.6 us instead of 45.8, weights as two fp16 terms 0.3e-4 to 1.6e-4 and 51.3 us.
   static constexpr bool kCentred = Pair<T>::kFine;
   uint32_t q[NT][2 * W][2];   // B fragments of the codes' product, two k-steps a group
   uint32_t qs[NT][2];         // and of the floors' product
@@ -1029,6 +1032,11 @@ int64_t scratch_bytes(const PagedInt4& p) {
 // 8.2; 2048: on eight 7.5, 8.6; 4096: on eight 9.4, 9.0.  Lengths are not known here, so a row has its
 // own CTAs only where the longest possible rows take less than the shortest shares, unless the rows are
 // known to be about equally long.  More clusters of eight than 112 CTAs do not run at once, of four 128.
+// Other shapes have other times and the same order, rows as long as the table, alone and by shares: 8 of 512
+// tokens, 4 x 64 (16 warps) 5.8 and 7.9 us, 16 heads on 1 x 128 (8 warps) 9.4 and 11.3, 16 on 1 x 64 7.3 and 9.6;
+// 8 of 2048, 7.4 (four CTAs) and 7.8, 10.6 (eight) and 13.0, 8.9 (eight) and 11.0.  Of 30 sizes a shape, 128..8192
+// tokens in 2..64 rows, the worst choice of CTAs was 8.7 us against 8.4 by shares (32 of 2048, 4 x 64); where the
+// shares are kept for want of the lengths, full rows would be up to 23 % sooner alone (64 of 1024, 16 on 1 x 64).
 int row_parts(int64_t rows, int64_t row_units, int warps, int ctas, bool even) {
   auto warp_units = [&](int64_t units) { return (units + warps - 1) / warps; };
   int64_t best = even ? 5 + 2 * warp_units((rows * (row_units + 1) + ctas - 1) / ctas) : 7;

@@ -56,7 +56,8 @@ __global__ void __launch_bounds__(kWriteThreads, write_ctas(ROPE)) int4_write_ke
   // Behind the wait: attention reads lengths and tables before its own, and what the kernel in front of
   // this one wrote is complete only now.
   // The kernel behind may stand by early where this one leaves the SMs at once (64 rows, then attention
-  // of 64 sequences: 24.5 us, else 25.1), but not beside the CTAs of a long grid (8192 rows 20.9 us, else 21.6).
+  // of 64 sequences: 24.5 us, else 24.6), but not beside the CTAs of a long grid (8192 rows written and read
+  // back 20.9 us, else 21.6).
   if (p.one_wave) release_dependents();
   const uint32_t first = blockIdx.x * kWriteThreads;
   const int index = first + threadIdx.x;

@@ -478,6 +478,9 @@ int launch_select(const PagedInt4& p, int head_dim, int dtype, bool last, cudaSt
   }
   QF_CUDA(err);
   const uint32_t* scored = keys;
+  // As few keys a thread as the table needs: bounds and sparse attention of 32 sequences with tables of 512 pages
+  // take 29.6 us with two a thread, 30.2 with five, 32.8 with sixteen; of one with 2049 pages, the 32768 tokens of a
+  // full context and the next, 17.3 with five and 20.0 with sixteen (four would hold 2048).
   if (p.table_width <= 2 * kPickThreads) {
     err = launch_chained(page_pick_kernel<2>, dim3(rows), dim3(kPickThreads), 0, stream, p, scored, last);
   } else if (p.table_width <= 5 * kPickThreads) {
