@@ -501,7 +501,9 @@ int qf_build_rope_table(float* table, int32_t positions, double base, void* stre
  * n * step + floor:
  *   floor = min(x)   step = T((max(x) - min(x)) / 15)   n = clamp(rint((x - floor) / step))
  * in fp32 with IEEE divisions, 5 bits a channel in all.  A step below 2^-60 is held as 0.
- * A group that holds an infinity or a NaN reads back as NaN.  Bytes of a tile, W = D / 32:
+ * A group that holds an infinity or a NaN, or whose range no finite fp32 number holds, reads
+ * back as NaN.  A step is rounded, so 15 * step + floor may lie beyond max(x), and beyond T's
+ * largest number, an infinity as T, where max(x) is next to that.  Bytes of a tile, W = D / 32:
  *   [0, 8D)     K codes [16 tokens][4 t][W][4]: byte y of (t, w): channels 32w + 8t + 2y (low
  *               four bits) and 32w + 8t + 2y + 1
  *   [8D, 16D)   V codes [8 token pairs][8 g][W][2 tokens][2]: byte y of (g, w): channels

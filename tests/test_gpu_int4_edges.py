@@ -110,3 +110,35 @@ def test_sparse_attention_takes_scales_from_zero_on(package, cuda_device):
         plain.assert_attention(out, *plain.attention(q, k, v, pages.cpu(), held.cpu(), scale))
     with pytest.raises(ValueError, match="scale"):
         package.sparse_decode_attention_int4(*call, num_pages=5, scale=-0.3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads, group, dim, page", [(2, 6, 128, 16), (1, 16, 64, 32)])
+@pytest.mark.parametrize("n", [20, 700, 5000])
+def test_queries_that_are_not_finite_stay_in_their_heads(package, cuda_device, dtype, heads, group, dim, page, n):
+    q, pool, table, lens = plain.make_cache([n, n, 3], dtype=dtype, dim=dim, heads=heads, group=group, page=page, seed=n)
+    want, top = plain.attention(q, *plain.rows(pool, dtype), table, lens)
+    q[0, 1, 5], q[1, group - 1, dim - 1], q[1, 0] = float("nan"), float("inf"), -float("inf")
+    out = package.paged_decode_attention_int4(*(t.to(cuda_device) for t in (q, pool, table, lens))).cpu()
+    spoiled = torch.zeros(out.shape, dtype=torch.bool)
+    spoiled[0, 1] = spoiled[1, group - 1] = spoiled[1, 0] = True
+    assert torch.equal(torch.isnan(out), spoiled)
+    plain.assert_attention(torch.where(spoiled, 0.0, out).to(dtype), torch.where(spoiled, 0.0, want), top)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_groups_at_the_ends_of_their_type(package, cuda_device, dtype):
+    """Rows whose groups reach the largest finite numbers, of one sign and of both."""
+    info = torch.finfo(dtype)
+    x = torch.zeros(16, 2, 128, dtype=dtype)
+    x[0, 0, 3], x[1, :, 40], x[2, 1, ::2], x[3] = info.max, -info.max, info.max, info.tiny
+    x[4, 0, 0], x[4, 0, 1] = info.max, -info.max
+    want = torch.zeros(1, 2, 1, 2560, dtype=torch.uint8)
+    plain.store(want, torch.arange(16), x, x)
+    got = package.quantize_kv_pool_int4(x[None].to(cuda_device), x[None].to(cuda_device))
+    k, v = (t.cpu()[0] for t in package.dequantize_kv_pool_int4(got, dtype))
+    value = plain.rows(want, dtype)[0][0].to(dtype)
+    wide = torch.zeros(16, 2, 128, dtype=torch.bool)
+    wide[4, 0, :32] = dtype is torch.bfloat16  # its range is beyond fp32
+    for back in (k, v):
+        assert torch.isnan(back)[wide].all() and torch.equal(back[~wide], value[~wide])
